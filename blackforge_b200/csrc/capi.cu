@@ -447,6 +447,79 @@ bfb_status bfb_attention_bwd(const void* d_dout, const void* d_q, const void* d_
     });
 }
 
+// ---- loss -----------------------------------------------------------------------------------------------
+
+bfb_status bfb_linear_cross_entropy_workspace(int32_t dtype, int64_t tokens, int64_t vocab, int64_t dim, int32_t backward,
+                                              size_t* bytes) {
+    return guarded([&] {
+        require(bytes != nullptr, "linear_cross_entropy_workspace: null result pointer");
+        *bytes = 0;
+        *bytes = bfb::linearCeWorkspaceBytes(dtype, tokens, vocab, dim, backward != 0);
+    });
+}
+
+bfb_status bfb_linear_cross_entropy_fwd(const void* d_x, int64_t ld_x, const void* d_w, int64_t ld_w, const float* d_bias,
+                                        const float* d_labels, float* d_loss, float* d_lse, float* d_summary, int32_t dtype,
+                                        int64_t tokens, int64_t vocab, int64_t dim, int32_t* d_oob_count, void* d_workspace,
+                                        size_t workspace_bytes, int32_t* d_status, void* stream) {
+    return guarded([&] {
+        bfb::LinearCeArgs a;
+        a.x = d_x;
+        a.ldX = ld_x;
+        a.w = d_w;
+        a.ldW = ld_w;
+        a.bias = d_bias;
+        a.labels = d_labels;
+        a.loss = d_loss;
+        a.lse = d_lse;
+        a.summary = d_summary;
+        a.dtype = dtype;
+        a.tokens = tokens;
+        a.vocab = vocab;
+        a.dim = dim;
+        a.oobCount = d_oob_count;
+        a.workspace = d_workspace;
+        a.workspaceBytes = workspace_bytes;
+        a.dStatus = d_status;
+        bfb::linearCeForward(a, asStream(stream));
+    });
+}
+
+bfb_status bfb_linear_cross_entropy_bwd(const void* d_x, int64_t ld_x, const void* d_w, int64_t ld_w, const float* d_bias,
+                                        const float* d_labels, const float* d_lse, const float* d_grad_loss,
+                                        const float* d_grad_scale, float grad_scale, void* d_dx, int64_t ld_dx, void* d_dw,
+                                        int64_t ld_dw, float* d_dbias, int32_t dtype, int32_t grad_dtype, int64_t tokens,
+                                        int64_t vocab, int64_t dim, void* d_workspace, size_t workspace_bytes,
+                                        int32_t* d_status, void* stream) {
+    return guarded([&] {
+        bfb::LinearCeArgs a;
+        a.x = d_x;
+        a.ldX = ld_x;
+        a.w = d_w;
+        a.ldW = ld_w;
+        a.bias = d_bias;
+        a.labels = d_labels;
+        a.lseIn = d_lse;
+        a.gradLoss = d_grad_loss;
+        a.dGradScale = d_grad_scale;
+        a.gradScale = grad_scale;
+        a.dx = d_dx;
+        a.ldDx = ld_dx;
+        a.dw = d_dw;
+        a.ldDw = ld_dw;
+        a.db = d_dbias;
+        a.dtype = dtype;
+        a.gradDtype = grad_dtype;
+        a.tokens = tokens;
+        a.vocab = vocab;
+        a.dim = dim;
+        a.workspace = d_workspace;
+        a.workspaceBytes = workspace_bytes;
+        a.dStatus = d_status;
+        bfb::linearCeBackward(a, asStream(stream));
+    });
+}
+
 // ---- model ----------------------------------------------------------------------------------------------
 
 static bfb_status createModel(const bfb_op_desc* ops, int32_t n_ops, int64_t input_last_dim, uint32_t seed,

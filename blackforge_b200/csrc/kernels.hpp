@@ -167,6 +167,46 @@ struct AttentionBackwardArgs {
 void attentionBackward(const AttentionBackwardArgs& args, cudaStream_t stream);
 bool attentionBackwardUsesTensorCores(const AttentionBackwardArgs& args);
 
+// Softmax cross entropy of z = x W^T + bias over a large vocabulary without keeping z, and its gradient (linear_ce.cu).
+struct LinearCeArgs {
+    const void* x = nullptr;           // [tokens, dim], row pitch ldX
+    const void* w = nullptr;           // [vocab, dim], row pitch ldW
+    const float* bias = nullptr;       // [vocab] or null
+    const float* labels = nullptr;     // [tokens]: class indices held in float32; negative = the row does not count
+    int64_t ldX = 0, ldW = 0;
+    int dtype = 0;                     // of x and w: BFB_F32 or BFB_BF16
+    int64_t tokens = 0, vocab = 0, dim = 0;
+    // forward
+    float* loss = nullptr;             // [tokens] or null
+    float* lse = nullptr;              // [tokens]
+    float* summary = nullptr;          // {sum of losses, counted rows, 1 / counted rows} or null
+    int* oobCount = nullptr;
+    // backward
+    const float* lseIn = nullptr;
+    const float* gradLoss = nullptr;   // [tokens] or null (1)
+    const float* dGradScale = nullptr; // one word on the device or null (1)
+    float gradScale = 1.0f;
+    void* dx = nullptr;                // [tokens, dim], row pitch ldDx; each of the three results may be null
+    void* dw = nullptr;                // [vocab, dim], row pitch ldDw
+    float* db = nullptr;               // [vocab]
+    int64_t ldDx = 0, ldDw = 0;
+    int gradDtype = 0;                 // of dx and dw
+    void* workspace = nullptr;         // linearCeWorkspaceBytes
+    size_t workspaceBytes = 0;
+    int* dStatus = nullptr;
+};
+size_t linearCeWorkspaceBytes(int dtype, int64_t tokens, int64_t vocab, int64_t dim, bool backward);
+bool linearCeUsesTensorCores(const LinearCeArgs& args);
+void linearCeForward(const LinearCeArgs& args, cudaStream_t stream);
+void linearCeBackward(const LinearCeArgs& args, cudaStream_t stream);
+// Its tensor-core products (linear_ce_tc.cu); callers have checked eligibility.
+void ceStatsTensorCore(const LinearCeArgs& a, float2* partials, float* labelLogit, cudaStream_t stream);
+void ceDzTensorCore(const LinearCeArgs& a, int64_t firstColumn, int64_t columns, void* dz, int64_t ldDz, float* biasPartials,
+                    cudaStream_t stream);
+void ceDxTensorCore(const LinearCeArgs& a, int64_t firstColumn, int64_t columns, const void* dz, int64_t ldDz, void* out, int outDtype,
+                    int64_t ldOut, const float* addend, int64_t ldAddend, cudaStream_t stream);
+void ceDwTensorCore(const LinearCeArgs& a, int64_t firstColumn, int64_t columns, const void* dz, int64_t ldDz, cudaStream_t stream);
+
 // Tensor-core kernels (gemm_tc.cu / attention_tc.cu); callers have checked eligibility.
 void gemmTensorCore(const GemmArgs& args, cudaStream_t stream);
 // CTA-pair variant (cta_group::2, 256 x 256 tiles); B must be [N,K].

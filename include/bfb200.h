@@ -310,6 +310,45 @@ bfb_status bfb_attention_bwd(const void* d_dout, const void* d_q, const void* d_
                              int64_t head_dim, int64_t ld_in, int64_t ld_kv, int64_t ld_grad_q, int64_t ld_grad_kv,
                              float scale, int64_t old_len, int32_t causal, int32_t* d_status, void* stream);
 
+/* ---- loss of a decoder: softmax cross entropy of its output projection --------------------------
+ * z = x W^T + bias, lse_t = log sum_v exp z_tv, loss_t = lse_t - z_t,label(t), without a tokens x vocab tensor of
+ * logits. Stands for linear / linearBf16 followed by softmaxCrossEntropySparse (src/backend/cuda/loss.cu:16-200) and for
+ * the gradients of both.
+ *  x [tokens, dim] and W [vocab, dim] (BFB_B_NK, as bfb_weight_prepare lays a weight out; a tied embedding table as it
+ *  is) have row pitches ld_x, ld_w in elements and one type: BFB_BF16 runs on the tensor cores (dim, ld_x and ld_w
+ *  multiples of 8, 16-byte aligned pointers; in the backward the same of the gradients), every other shape and
+ *  BFB_F32 on CUDA cores with fp32 products. bias f32 [vocab] may be NULL; -inf there takes a class out.
+ *  labels are float32 holding integers, rounded to the nearest, as token ids are everywhere. A negative label takes the
+ *  row out (loss 0, no gradient). One at or above vocab, or not finite, does the same and increments *d_oob_count
+ *  (optional, int32 on device): the host layer turns a non-zero count into BFB_INVALID_ARGUMENT.
+ *  Sums and statistics are fp32 or wider and added in a fixed order: the same bits on every run. A row whose logits are
+ *  all -inf, or hold +inf or NaN, has no distribution: its loss and its gradient are NaN. x has to be finite in rows that
+ *  do not count, too: they meet their zero gradient in the product that gives dW.
+ *  d_status (optional int32 on device) as for bfb_gemm.
+ * _workspace: bytes of the caller's workspace for a forward (backward == 0) or for both directions. It holds one piece of
+ * the vocabulary's gradient of z (tokens x piece, at most 256 MiB or 4096 columns) and fp32 sums of dx; its pointer has to be
+ * 256-byte aligned. Nothing in it has to survive from call to call, and nothing of it is kept: calls that may run at the
+ * same time (other streams, two captured graphs) take one each.
+ * _fwd writes d_loss [tokens] (may be NULL), d_lse [tokens] and, when d_summary is not NULL, {sum of the losses, rows that
+ * count, 1 / rows that count (0 if none)}.
+ * _bwd takes the same operands and d_lse, and the gradient of each row's loss as grad_scale * *d_grad_scale *
+ * d_grad_loss[t] (the two device operands may be NULL, standing for 1): d_grad_scale = d_summary + 2 gives the mean's
+ * gradient. Each of d_dx [tokens, dim], d_dw [vocab, dim] (grad_dtype BFB_F32 or BFB_BF16, pitches ld_dx, ld_dw) and
+ * d_dbias f32 [vocab] may be NULL and is overwritten otherwise. On the tensor-core route the gradient of z is rounded to bf16
+ * once, as the operand of the two products (dbias sums the unrounded values). */
+bfb_status bfb_linear_cross_entropy_workspace(int32_t dtype, int64_t tokens, int64_t vocab, int64_t dim, int32_t backward,
+                                              size_t* bytes);
+bfb_status bfb_linear_cross_entropy_fwd(const void* d_x, int64_t ld_x, const void* d_w, int64_t ld_w, const float* d_bias,
+                                        const float* d_labels, float* d_loss, float* d_lse, float* d_summary, int32_t dtype,
+                                        int64_t tokens, int64_t vocab, int64_t dim, int32_t* d_oob_count, void* d_workspace,
+                                        size_t workspace_bytes, int32_t* d_status, void* stream);
+bfb_status bfb_linear_cross_entropy_bwd(const void* d_x, int64_t ld_x, const void* d_w, int64_t ld_w, const float* d_bias,
+                                        const float* d_labels, const float* d_lse, const float* d_grad_loss,
+                                        const float* d_grad_scale, float grad_scale, void* d_dx, int64_t ld_dx, void* d_dw,
+                                        int64_t ld_dw, float* d_dbias, int32_t dtype, int32_t grad_dtype, int64_t tokens,
+                                        int64_t vocab, int64_t dim, void* d_workspace, size_t workspace_bytes,
+                                        int32_t* d_status, void* stream);
+
 /* ---- model: the IR executor's device side ------------------------------------------------------
  * Replaces cuda::Model (src/backend/cuda/model.cu:139-306: constructor, forward, parameters),
  * cuda::Executor::run / makeSyntheticInput (src/backend/cuda/executor.cu:26-132) and
