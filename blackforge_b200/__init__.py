@@ -100,6 +100,10 @@ SIGNATURES = {
     "bfb_linear_cross_entropy_fwd": (_I32, [_P, _I64, _P, _I64, _P, _P, _P, _P, _P, _I32, _I64, _I64, _I64, _P, _P, _SZ, _P, _P]),
     "bfb_linear_cross_entropy_bwd": (_I32, [_P, _I64, _P, _I64, _P, _P, _P, _P, _P, _F, _P, _I64, _P, _I64, _P, _I32, _I32, _I64,
                                             _I64, _I64, _P, _SZ, _P, _P]),
+    "bfb_embed_scaled": (_I32, [_P, _P, _I32, _P, _I32, _I64, _I64, _I64, _I64, _F, _P, _P]),
+    "bfb_embed_scaled_bwd_workspace": (_I32, [_I64, _I64, _I64, C.POINTER(_SZ)]),
+    "bfb_embed_scaled_bwd": (_I32, [_P, _P, _I32, _I64, _P, _I32, _I64, _I64, _I64, _F, _I32, _P, _SZ, _P]),
+    "bfb_distill_topk": (_I32, [_P, _I32, _I64, _P, _P, _I32, _I64, _F, _P, _P, _F, _P, _P, _P, _I32, _I64, _I64, _I64, _P, _P]),
     "bfb_model_create": (_I32, [C.POINTER(OpDesc), _I32, _I64, C.c_uint32, C.POINTER(Precision), C.POINTER(_P)]),
     "bfb_model_create_uninitialised": (_I32, [C.POINTER(OpDesc), _I32, _I64, C.POINTER(Precision), C.POINTER(_P)]),
     "bfb_model_destroy": (None, [_P]),

@@ -31,6 +31,8 @@ SOURCES = [
     "attention_tc.cu",
     "attention_bwd.cu",
     "attention_decode.cu",
+    "embed_grad.cu",
+    "distill.cu",
     "linear_ce.cu",
     "linear_ce_tc.cu",
     "selftest.cu",

@@ -520,6 +520,61 @@ bfb_status bfb_linear_cross_entropy_bwd(const void* d_x, int64_t ld_x, const voi
     });
 }
 
+bfb_status bfb_embed_scaled(const float* d_ids, const void* d_table, int32_t table_dtype, void* d_out, int32_t out_dtype,
+                            int64_t ld_out, int64_t tokens, int64_t vocab, int64_t dim, float scale, int32_t* d_oob_count,
+                            void* stream) {
+    return guarded([&] {
+        bfb::embedScaled(d_ids, d_table, table_dtype, d_out, out_dtype, ld_out, tokens, vocab, dim, scale, d_oob_count, asStream(stream));
+    });
+}
+
+bfb_status bfb_embed_scaled_bwd_workspace(int64_t tokens, int64_t vocab, int64_t dim, size_t* bytes) {
+    return guarded([&] {
+        require(bytes != nullptr, "embed_scaled_bwd_workspace: null result pointer");
+        *bytes = 0;
+        *bytes = bfb::embedScaledBackwardWorkspaceBytes(tokens, vocab, dim);
+    });
+}
+
+bfb_status bfb_embed_scaled_bwd(const float* d_ids, const void* d_dout, int32_t dout_dtype, int64_t ld_dout, void* d_dtable,
+                                int32_t dtable_dtype, int64_t tokens, int64_t vocab, int64_t dim, float scale,
+                                int32_t accumulate, void* d_workspace, size_t workspace_bytes, void* stream) {
+    return guarded([&] {
+        bfb::embedScaledBackward(d_ids, d_dout, dout_dtype, ld_dout, d_dtable, dtable_dtype, tokens, vocab, dim, scale, accumulate != 0,
+                                 d_workspace, workspace_bytes, asStream(stream));
+    });
+}
+
+bfb_status bfb_distill_topk(const void* d_logits, int32_t dtype, int64_t ld_logits, const float* d_teacher_ids,
+                            const void* d_teacher_logits, int32_t teacher_dtype, int64_t k, float temperature,
+                            const float* d_grad_loss, const float* d_grad_scale, float grad_scale, float* d_loss,
+                            float* d_lse, void* d_dlogits, int32_t grad_dtype, int64_t ld_dlogits, int64_t rows,
+                            int64_t vocab, int32_t* d_oob_count, void* stream) {
+    return guarded([&] {
+        bfb::DistillArgs a;
+        a.logits = d_logits;
+        a.dtype = dtype;
+        a.ldLogits = ld_logits;
+        a.ids = d_teacher_ids;
+        a.teacher = d_teacher_logits;
+        a.teacherDtype = teacher_dtype;
+        a.k = k;
+        a.tau = temperature;
+        a.gradLoss = d_grad_loss;
+        a.dGradScale = d_grad_scale;
+        a.gradScale = grad_scale;
+        a.loss = d_loss;
+        a.lse = d_lse;
+        a.grad = d_dlogits;
+        a.gradDtype = grad_dtype;
+        a.ldGrad = ld_dlogits;
+        a.rows = rows;
+        a.vocab = vocab;
+        a.oobCount = d_oob_count;
+        bfb::distillTopk(a, asStream(stream));
+    });
+}
+
 // ---- model ----------------------------------------------------------------------------------------------
 
 static bfb_status createModel(const bfb_op_desc* ops, int32_t n_ops, int64_t input_last_dim, uint32_t seed,

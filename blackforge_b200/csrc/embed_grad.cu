@@ -1,0 +1,541 @@
+// Embedding lookup with a scale, and the gradient of the table by sorted tokens.
+//
+//   out_t = scale * E[id_t],      dE_v = scale * sum_{t: id_t = v} dout_t
+//
+// Both are bound by memory. The gradient reads dout once and writes the table once, with no atomics, so that its bits do not
+// depend on timing:
+//   1. sortTokensKernel orders the token positions by id (stable: positions of one id stay ascending). One cluster of up
+//      to eight blocks does all digits of a radix sort in one launch, its counters joined over distributed shared memory.
+//   2. embedReduceKernel cuts the sorted list into pieces of equal length whatever ids they hold, so that a token that makes
+//      up a third of the text costs what any other rows cost. A block sums a piece's rows in fp32 and stores each id whose
+//      whole run lies inside; the ends of runs that cross a border go to a small array. Other blocks of the same launch
+//      write the rows of ids that do not occur.
+//   3. embedJoinKernel adds up the parts of the runs that crossed borders, in order.
+#include <cuda_bf16.h>
+
+#include <algorithm>
+#include <climits>
+
+#include "common.cuh"
+#include "kernels.hpp"
+#include "ptx_sm100.cuh"
+
+namespace bfb {
+
+namespace {
+
+constexpr int kSortThreads = 1024;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kSortCluster = 8;
+constexpr int kMaxDigitBits = 9;
+constexpr int kMaxPiece = 128;      // most sorted entries per block of the reduction
+constexpr int kZeroRows = 64;       // table rows a block looks after when it writes the rows that do not occur
+constexpr int kReduceThreads = 256;
+
+inline int64_t roundUp(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+inline bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// Token ids are float32 holding integers; one outside [0, vocab) names no row.
+__device__ __forceinline__ uint32_t tokenRow(float idf, int64_t vocab) {
+    if (!(fabsf(idf) < 2147483648.0f)) return static_cast<uint32_t>(vocab);
+    const int64_t id = static_cast<int64_t>(lroundf(idf));
+    return id >= 0 && id < vocab ? static_cast<uint32_t>(id) : static_cast<uint32_t>(vocab);
+}
+
+template <typename T>
+__device__ __forceinline__ float toFloat(T v);
+template <>
+__device__ __forceinline__ float toFloat<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float toFloat<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T fromFloat(float v);
+template <>
+__device__ __forceinline__ float fromFloat<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 fromFloat<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// kN neighbouring elements, aligned to their size up to 16 bytes.
+template <typename T, int kN>
+struct alignas(sizeof(T) * kN < 16 ? sizeof(T) * kN : 16) Pack {
+    T v[kN];
+};
+
+// ---- lookup --------------------------------------------------------------------------------------------------
+
+// blockDim.x threads across a row's packs, blockDim.y tokens per block.
+template <typename TIn, typename TOut, int kN>
+__global__ void __launch_bounds__(256)
+embedScaledKernel(const float* __restrict__ ids, const TIn* __restrict__ table, TOut* __restrict__ out, int64_t ldOut, int64_t tokens,
+                  int64_t vocab, int64_t dim, float scale, int* oobCount) {
+    const int64_t packs = dim / kN;
+    for (int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y; t < tokens; t += static_cast<int64_t>(gridDim.x) * blockDim.y) {
+        const uint32_t id = tokenRow(ids[t], vocab);
+        const bool ok = id < vocab;
+        if (!ok && threadIdx.x == 0 && oobCount != nullptr) atomicAdd(oobCount, 1);
+        const auto* src = reinterpret_cast<const Pack<TIn, kN>*>(table + static_cast<int64_t>(ok ? id : 0) * dim);
+        auto* dst = reinterpret_cast<Pack<TOut, kN>*>(out + t * ldOut);
+        for (int64_t i = threadIdx.x; i < packs; i += blockDim.x) {
+            Pack<TOut, kN> r;
+            if (ok) {
+                const Pack<TIn, kN> v = src[i];
+#pragma unroll
+                for (int j = 0; j < kN; ++j) r.v[j] = fromFloat<TOut>(toFloat(v.v[j]) * scale);
+            } else {
+#pragma unroll
+                for (int j = 0; j < kN; ++j) r.v[j] = fromFloat<TOut>(0.0f);
+            }
+            dst[i] = r;
+        }
+    }
+}
+
+// ---- 1. sort -------------------------------------------------------------------------------------------------
+
+struct SortBuffers {
+    uint32_t* keys[2];
+    uint32_t* values[2];
+};
+
+// Stable radix sort of (row, position) pairs, `passes` digits of `bits` bits. The cluster's blocks, their warps and a
+// warp's batches of 32 take consecutive stretches of the list; a pair's place is: all smaller digits, the same digit in
+// stretches before its own, the same digit before it in its batch. Rows that name no id (vocab) end up last.
+__global__ void __launch_bounds__(kSortThreads, 1)
+sortTokensKernel(const float* __restrict__ ids, SortBuffers buf, int64_t count, int64_t vocab, int passes, int bits, int cluster) {
+    extern __shared__ uint32_t counts[];   // [kSortWarps][bins], then [bins] totals of this block, [bins] bases
+    const int bins = 1 << bits;
+    uint32_t* blockTotal = counts + kSortWarps * bins;
+    uint32_t* base = blockTotal + bins;
+    __shared__ uint32_t warpScan[kSortWarps];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rank = static_cast<int>(cluster_ctarank());
+    const int64_t perWarp = (count + static_cast<int64_t>(cluster) * kSortWarps * 32 - 1) / (static_cast<int64_t>(cluster) * kSortWarps * 32) * 32;
+    const int64_t begin = min(count, (static_cast<int64_t>(rank) * kSortWarps + warp) * perWarp);
+    const int64_t end = min(count, begin + perWarp);
+    uint32_t* mine = counts + warp * bins;
+
+    for (int pass = 0; pass < passes; ++pass) {
+        const int shift = pass * bits;
+        const uint32_t* srcKeys = buf.keys[(pass & 1) ^ 1];
+        const uint32_t* srcValues = buf.values[(pass & 1) ^ 1];
+        uint32_t* dstKeys = buf.keys[pass & 1];
+        uint32_t* dstValues = buf.values[pass & 1];
+        auto keyAt = [&](int64_t i) { return pass == 0 ? tokenRow(ids[i], vocab) : __ldcg(srcKeys + i); };
+        for (int i = tid; i < kSortWarps * bins; i += kSortThreads) counts[i] = 0;
+        __syncthreads();
+        for (int64_t i = begin + lane; i < end; i += 32) atomicAdd(&mine[(keyAt(i) >> shift) & (bins - 1)], 1u);
+        __syncthreads();
+        // per digit: what the block's earlier warps hold, and the block's total
+        if (tid < bins) {
+            uint32_t total = 0;
+            for (int w = 0; w < kSortWarps; ++w) {
+                const uint32_t n = counts[w * bins + tid];
+                counts[w * bins + tid] = total;
+                total += n;
+            }
+            blockTotal[tid] = total;
+        }
+        if (cluster > 1) cluster_sync_all();
+        else __syncthreads();
+        // per digit: all blocks' totals, and those of the blocks before this one
+        uint32_t all = 0, before = 0;
+        if (tid < bins) {
+            for (int r = 0; r < cluster; ++r) {
+                uint32_t n;
+                const uint32_t from = mapa_cluster(smem_u32(&blockTotal[tid]), static_cast<uint32_t>(r));
+                asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(n) : "r"(from) : "memory");
+                all += n;
+                before += r < rank ? n : 0;
+            }
+        }
+        uint32_t scan = all;   // inclusive over the digits
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t n = __shfl_up_sync(0xFFFFFFFFu, scan, o);
+            if (lane >= o) scan += n;
+        }
+        if (lane == 31) warpScan[warp] = scan;
+        __syncthreads();
+        uint32_t smaller = 0;
+        for (int w = 0; w < warp; ++w) smaller += warpScan[w];
+        if (tid < bins) base[tid] = smaller + scan - all + before;
+        __syncthreads();
+        // places, 32 pairs at a time
+        for (int64_t i0 = begin; i0 < end; i0 += 32) {
+            const int64_t i = i0 + lane;
+            const bool live = i < end;
+            const uint32_t key = live ? keyAt(i) : 0;
+            const uint32_t value = live ? (pass == 0 ? static_cast<uint32_t>(i) : __ldcg(srcValues + i)) : 0;
+            const uint32_t digit = live ? (key >> shift) & (bins - 1) : 0xFFFFFFFFu;
+            const uint32_t same = __match_any_sync(0xFFFFFFFFu, digit);
+            if (live) {
+                const uint32_t earlier = __popc(same & ((1u << lane) - 1u));
+                const uint32_t at = base[digit] + mine[digit] + earlier;
+                if (at < count) {   // always, unless the ids change while the kernel runs
+                    dstKeys[at] = key;
+                    dstValues[at] = value;
+                }
+            }
+            __syncwarp();
+            if (live && lane == 31 - __clz(same)) mine[digit] += __popc(same);
+            __syncwarp();
+        }
+        // the next pass reads what other blocks wrote; and nobody leaves while its totals are being read
+        __threadfence();
+        if (cluster > 1) cluster_sync_all();
+        else __syncthreads();
+    }
+}
+
+// ---- 2. sums of the sorted rows ---------------------------------------------------------------------------------
+
+struct ReduceParams {
+    const uint32_t* keys;      // sorted rows
+    const uint32_t* values;    // token positions
+    int64_t count;             // entries, those that name no row last
+    int64_t vocab, dim;
+    const void* dout;
+    int64_t ldDout;
+    void* dtable;
+    float scale;
+    int accumulate;
+    float* ends;               // [pieces][2][dim]: sums of a piece's first run (begun earlier) and last run (going on)
+    int64_t pieces;
+    int piece;                 // entries a piece
+    int64_t columnBlocks;
+};
+
+template <typename T, int kN>
+__device__ __forceinline__ void storeRow(T* row, int64_t pack, const float (&acc)[kN], float scale, bool accumulate) {
+    auto* dst = reinterpret_cast<Pack<T, kN>*>(row) + pack;
+    Pack<T, kN> r;
+    if (accumulate) {
+        const Pack<T, kN> old = *dst;
+#pragma unroll
+        for (int j = 0; j < kN; ++j) r.v[j] = fromFloat<T>(fmaf(acc[j], scale, toFloat(old.v[j])));
+    } else {
+#pragma unroll
+        for (int j = 0; j < kN; ++j) r.v[j] = fromFloat<T>(acc[j] * scale);
+    }
+    *dst = r;
+}
+
+template <typename TIn, typename TOut, int kN>
+__global__ void __launch_bounds__(kReduceThreads)
+embedReduceKernel(const ReduceParams p) {
+    __shared__ uint32_t sKey[kMaxPiece + 2], sValue[kMaxPiece];
+    const int64_t reduceBlocks = p.pieces * p.columnBlocks;
+    const int tid = threadIdx.x;
+    if (blockIdx.x < reduceBlocks) {
+        const int64_t piece = blockIdx.x / p.columnBlocks;
+        const int64_t pack = (blockIdx.x % p.columnBlocks) * kReduceThreads + tid;
+        const int64_t begin = piece * p.piece;
+        const int n = static_cast<int>(min(static_cast<int64_t>(p.piece), p.count - begin));
+        // the piece with its neighbours on both sides; `vocab` stands for no row
+        const uint32_t none = static_cast<uint32_t>(p.vocab);
+        if (tid < n + 2) {
+            const int64_t i = begin + tid - 1;
+            sKey[tid] = i >= 0 && i < p.count ? p.keys[i] : none;
+            if (tid >= 1 && tid <= n) sValue[tid - 1] = p.values[i];
+        }
+        __syncthreads();
+        if (pack * kN >= p.dim) return;
+        const TIn* dout = static_cast<const TIn*>(p.dout) + pack * kN;
+        TOut* table = static_cast<TOut*>(p.dtable);
+        float acc[kN] = {};
+        int runBegin = 0;
+        auto flush = [&](int runEnd) {   // entries [runBegin, runEnd) of the piece are one run
+            const uint32_t key = sKey[runBegin + 1];
+            const bool begun = runBegin == 0 && sKey[0] == key;
+            const bool goesOn = runEnd == n && sKey[n + 1] == key;
+            if (begun || goesOn) {
+                float* end = p.ends + (piece * 2 + (begun ? 0 : 1)) * p.dim + pack * kN;
+#pragma unroll
+                for (int j = 0; j < kN; ++j) end[j] = acc[j];
+            } else {
+                storeRow<TOut, kN>(table + static_cast<int64_t>(key) * p.dim, pack, acc, p.scale, p.accumulate != 0);
+            }
+        };
+        constexpr int kAhead = 8;
+        for (int i0 = 0; i0 < n; i0 += kAhead) {
+            Pack<TIn, kN> v[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                if (i0 + u < n && sKey[i0 + u + 1] != none)
+                    v[u] = *reinterpret_cast<const Pack<TIn, kN>*>(dout + static_cast<int64_t>(sValue[i0 + u]) * p.ldDout);
+            }
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const int i = i0 + u;
+                if (i >= n || sKey[i + 1] == none) break;
+                if (i > runBegin && sKey[i + 1] != sKey[i]) {
+                    flush(i);
+                    runBegin = i;
+#pragma unroll
+                    for (int j = 0; j < kN; ++j) acc[j] = 0.0f;
+                }
+#pragma unroll
+                for (int j = 0; j < kN; ++j) acc[j] += toFloat(v[u].v[j]);
+            }
+        }
+        // the last run ends with the piece or where the entries without a row begin
+        int live = n;
+        while (live > 0 && sKey[live] == none) --live;
+        if (live > 0) {
+            if (live == n) {
+                flush(n);
+            } else {
+                const uint32_t key = sKey[runBegin + 1];
+                if (runBegin == 0 && sKey[0] == key) {
+                    float* end = p.ends + piece * 2 * p.dim + pack * kN;
+#pragma unroll
+                    for (int j = 0; j < kN; ++j) end[j] = acc[j];
+                } else {
+                    storeRow<TOut, kN>(table + static_cast<int64_t>(key) * p.dim, pack, acc, p.scale, p.accumulate != 0);
+                }
+            }
+        }
+        return;
+    }
+    // ---- rows that do not occur: a block looks after kZeroRows neighbouring rows
+    __shared__ uint32_t seen[kZeroRows / 32];
+    const int64_t row0 = (blockIdx.x - reduceBlocks) * kZeroRows;
+    const int rows = static_cast<int>(min(static_cast<int64_t>(kZeroRows), p.vocab - row0));
+    if (tid < kZeroRows / 32) seen[tid] = 0;
+    __syncthreads();
+    // first sorted entry at or above row0: every warp narrows the range to a 33rd per step
+    int64_t low = 0, high = p.count;
+    while (low < high) {
+        const int64_t probe = low + (high - low) * (tid & 31) / 32;
+        const int below = __popc(__ballot_sync(0xFFFFFFFFu, p.keys[probe] < row0));   // the probes ascend
+        const int64_t next = low + (high - low) * below / 32;                         // first probe that is not below (or high)
+        const int64_t before = low + (high - low) * (below - 1) / 32;
+        if (below > 0) low = before + 1;
+        high = below == 0 ? low : next;
+    }
+    for (int64_t i = low + tid;; i += blockDim.x) {
+        const uint32_t key = i < p.count ? p.keys[i] : static_cast<uint32_t>(p.vocab);
+        const bool inside = key < static_cast<uint64_t>(row0) + rows && key < p.vocab;
+        if (inside) atomicOr(&seen[(key - row0) >> 5], 1u << ((key - row0) & 31));
+        if (__syncthreads_and(inside) == 0) break;
+    }
+    TOut* table = static_cast<TOut*>(p.dtable);
+    int r = 0;
+    while (r < rows) {
+        if ((seen[r >> 5] >> (r & 31)) & 1u) {
+            ++r;
+            continue;
+        }
+        int to = r + 1;   // a stretch of rows without a token is one stretch of memory
+        while (to < rows && !((seen[to >> 5] >> (to & 31)) & 1u)) ++to;
+        char* from = reinterpret_cast<char*>(table + (row0 + r) * p.dim);
+        const int64_t bytes = static_cast<int64_t>(to - r) * p.dim * static_cast<int64_t>(sizeof(TOut));
+        const int64_t head = min(bytes, static_cast<int64_t>((16 - reinterpret_cast<uintptr_t>(from) % 16) % 16));
+        const int64_t body = (bytes - head) / 16;
+        for (int64_t i = tid; i < head / static_cast<int64_t>(sizeof(TOut)); i += blockDim.x) reinterpret_cast<TOut*>(from)[i] = fromFloat<TOut>(0.0f);
+        for (int64_t i = tid; i < body; i += blockDim.x) __stcs(reinterpret_cast<uint4*>(from + head) + i, make_uint4(0, 0, 0, 0));
+        for (int64_t i = head + body * 16 + tid * static_cast<int64_t>(sizeof(TOut)); i < bytes; i += blockDim.x * static_cast<int64_t>(sizeof(TOut)))
+            *reinterpret_cast<TOut*>(from + i) = fromFloat<TOut>(0.0f);
+        r = to;
+    }
+}
+
+// ---- 3. runs that cross the borders of pieces --------------------------------------------------------------------
+
+// A piece whose last run goes on, and did not begin before the piece, starts a chain: its own part, then the first parts of
+// the pieces behind it that begin with the same row. One column per thread, parts added in order, eight in flight.
+template <typename TOut>
+__global__ void __launch_bounds__(256)
+embedJoinKernel(const ReduceParams p) {
+    const int64_t piece = blockIdx.x;
+    const int64_t begin = piece * p.piece, next = begin + p.piece;   // piece + 1 < pieces: `next` is an entry
+    const uint32_t key = p.keys[next - 1], following = p.keys[next], first = p.keys[begin], earlier = begin > 0 ? p.keys[begin - 1] : 0xFFFFFFFFu;
+    if (key >= p.vocab || following != key) return;       // nothing goes on
+    if (first == key && earlier == key) return;           // the chain started earlier
+    const int64_t col = static_cast<int64_t>(blockIdx.y) * blockDim.x + threadIdx.x;
+    if (col >= p.dim) return;
+    constexpr int kAhead = 8;
+    float sum = p.ends[(piece * 2 + 1) * p.dim + col];
+    for (int64_t q = piece + 1;; q += kAhead) {
+        bool in[kAhead];
+        float part[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) in[u] = q + u < p.pieces && p.keys[(q + u) * p.piece] == key;
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) part[u] = in[u] ? p.ends[(q + u) * 2 * p.dim + col] : 0.0f;
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) sum += part[u];
+        if (!in[kAhead - 1]) break;
+    }
+    const float acc[1] = {sum};
+    storeRow<TOut, 1>(static_cast<TOut*>(p.dtable) + static_cast<int64_t>(key) * p.dim, col, acc, p.scale, p.accumulate != 0);
+}
+
+struct SortPlan {
+    int passes, bits, cluster;
+};
+SortPlan sortPlan(int64_t tokens, int64_t vocab) {
+    int width = 1;
+    while ((1ll << width) <= vocab) ++width;   // rows 0 .. vocab - 1, and vocab for "none"
+    SortPlan s;
+    s.passes = (width + kMaxDigitBits - 1) / kMaxDigitBits;
+    s.bits = (width + s.passes - 1) / s.passes;
+    s.cluster = tokens <= 4096 ? 1 : kSortCluster;
+    return s;
+}
+
+struct EmbedWorkspace {
+    size_t list, ends, total;
+    int piece;
+    int64_t pieces;
+};
+// Entries per piece: as many as leave eight blocks for each of 148 SMs (the ends of a piece cost two rows of fp32, so long
+// pieces move less), between 8 and 128.
+EmbedWorkspace embedWorkspace(int64_t tokens, int64_t dim) {
+    EmbedWorkspace w;
+    const int64_t share = tokens * ((dim + 1023) / 1024) / (148 * 8);
+    w.piece = 8;
+    while (w.piece * 2 <= std::min<int64_t>(share, kMaxPiece)) w.piece *= 2;
+    w.pieces = (tokens + w.piece - 1) / w.piece;
+    w.list = static_cast<size_t>(roundUp(std::max<int64_t>(tokens, 1) * 4, 256));
+    w.ends = static_cast<size_t>(roundUp(w.pieces * 2 * dim * 4, 256));
+    w.total = 4 * w.list + w.ends;
+    return w;
+}
+
+template <typename TIn, typename TOut, int kN>
+void launchReduce(ReduceParams p, cudaStream_t stream) {
+    p.columnBlocks = (p.dim / kN + kReduceThreads - 1) / kReduceThreads;
+    const int64_t zeroBlocks = p.accumulate ? 0 : (p.vocab + kZeroRows - 1) / kZeroRows;
+    const int64_t blocks = p.pieces * p.columnBlocks + zeroBlocks;
+    if (blocks > 0) {
+        embedReduceKernel<TIn, TOut, kN><<<static_cast<unsigned>(blocks), kReduceThreads, 0, stream>>>(p);
+        BFB_LAUNCH_CHECK();
+        noteLaunch();
+    }
+    if (p.pieces > 1) {
+        const dim3 grid(static_cast<unsigned>(p.pieces - 1), static_cast<unsigned>((p.dim + 255) / 256));
+        embedJoinKernel<TOut><<<grid, 256, 0, stream>>>(p);
+        BFB_LAUNCH_CHECK();
+        noteLaunch();
+    }
+}
+
+template <typename TIn, typename TOut>
+void reduceAnyPack(const ReduceParams& p, cudaStream_t stream) {
+    constexpr int kWide = 16 / static_cast<int>(sizeof(TIn));
+    const bool wide = p.dim % kWide == 0 && p.ldDout % kWide == 0 && aligned16(p.dout) && aligned16(p.dtable) && p.dim * sizeof(TOut) % 16 == 0;
+    if (wide) launchReduce<TIn, TOut, kWide>(p, stream);
+    else launchReduce<TIn, TOut, 1>(p, stream);
+}
+
+template <typename TIn, typename TOut>
+void launchLookup(const float* ids, const void* table, void* out, int64_t ldOut, int64_t tokens, int64_t vocab, int64_t dim, float scale,
+                  int* oobCount, cudaStream_t stream) {
+    constexpr int kWide = sizeof(TIn) == 2 && sizeof(TOut) == 2 ? 8 : 4;
+    const bool wide = dim % kWide == 0 && ldOut % kWide == 0 && aligned16(table) && aligned16(out);
+    const int64_t packs = wide ? dim / kWide : dim;
+    const int across = static_cast<int>(std::min<int64_t>(256, roundUp(packs, 32)));
+    const dim3 block(across, 256 / across);
+    const int64_t blocks = (tokens + block.y - 1) / block.y;
+    const int grid = static_cast<int>(std::min<int64_t>(blocks, static_cast<int64_t>(smCount()) * 32));
+    const auto* t = static_cast<const TIn*>(table);
+    auto* o = static_cast<TOut*>(out);
+    if (wide) embedScaledKernel<TIn, TOut, kWide><<<grid, block, 0, stream>>>(ids, t, o, ldOut, tokens, vocab, dim, scale, oobCount);
+    else embedScaledKernel<TIn, TOut, 1><<<grid, block, 0, stream>>>(ids, t, o, ldOut, tokens, vocab, dim, scale, oobCount);
+    BFB_LAUNCH_CHECK();
+    noteLaunch();
+}
+
+void checkSizes(int64_t tokens, int64_t vocab, int64_t dim) {
+    require(tokens >= 0 && vocab > 0 && dim > 0, "embed_scaled: sizes must be positive");
+    require(tokens < (1ll << 31) && vocab <= (1ll << 24) && dim <= (1ll << 20), "embed_scaled: sizes beyond the limits (2^31 tokens, 2^24 rows, 2^20 columns)");
+}
+
+}  // namespace
+
+void embedScaled(const float* ids, const void* table, int tableDtype, void* out, int outDtype, int64_t ldOut, int64_t tokens, int64_t vocab,
+                 int64_t dim, float scale, int* oobCount, cudaStream_t stream) {
+    checkSizes(tokens, vocab, dim);
+    require(tableDtype == BFB_F32 || tableDtype == BFB_BF16, "embed_scaled: the table must be f32 or bf16");
+    require(outDtype == BFB_F32 || outDtype == BFB_BF16, "embed_scaled: the output must be f32 or bf16");
+    require(ldOut >= dim, "embed_scaled: row pitch smaller than dim");
+    if (tokens == 0) return;
+    require(ids != nullptr && table != nullptr && out != nullptr, "embed_scaled: null pointer");
+    using bf = __nv_bfloat16;
+    if (tableDtype == BFB_F32) {
+        if (outDtype == BFB_F32) launchLookup<float, float>(ids, table, out, ldOut, tokens, vocab, dim, scale, oobCount, stream);
+        else launchLookup<float, bf>(ids, table, out, ldOut, tokens, vocab, dim, scale, oobCount, stream);
+    } else {
+        if (outDtype == BFB_F32) launchLookup<bf, float>(ids, table, out, ldOut, tokens, vocab, dim, scale, oobCount, stream);
+        else launchLookup<bf, bf>(ids, table, out, ldOut, tokens, vocab, dim, scale, oobCount, stream);
+    }
+}
+
+size_t embedScaledBackwardWorkspaceBytes(int64_t tokens, int64_t vocab, int64_t dim) {
+    checkSizes(tokens, vocab, dim);
+    return embedWorkspace(tokens, dim).total;
+}
+
+void embedScaledBackward(const float* ids, const void* dout, int doutDtype, int64_t ldDout, void* dtable, int dtableDtype, int64_t tokens,
+                         int64_t vocab, int64_t dim, float scale, bool accumulate, void* workspace, size_t workspaceBytes,
+                         cudaStream_t stream) {
+    checkSizes(tokens, vocab, dim);
+    require(doutDtype == BFB_F32 || doutDtype == BFB_BF16, "embed_scaled_bwd: the gradient must be f32 or bf16");
+    require(dtableDtype == BFB_F32 || dtableDtype == BFB_BF16, "embed_scaled_bwd: the table's gradient must be f32 or bf16");
+    require(ldDout >= dim, "embed_scaled_bwd: row pitch smaller than dim");
+    require(dtable != nullptr, "embed_scaled_bwd: null pointer");
+    if (tokens > 0) require(ids != nullptr && dout != nullptr, "embed_scaled_bwd: null pointer");
+    const EmbedWorkspace need = embedWorkspace(tokens, dim);
+    require(tokens == 0 || (workspace != nullptr && workspaceBytes >= need.total && reinterpret_cast<uintptr_t>(workspace) % 256 == 0),
+            "embed_scaled_bwd: the workspace is missing, too small (bfb_embed_scaled_bwd_workspace) or not 256-byte aligned");
+    ReduceParams p{};
+    p.count = tokens;
+    p.vocab = vocab;
+    p.dim = dim;
+    p.dout = dout;
+    p.ldDout = ldDout;
+    p.dtable = dtable;
+    p.scale = scale;
+    p.accumulate = accumulate ? 1 : 0;
+    p.piece = need.piece;
+    p.pieces = need.pieces;
+    if (tokens > 0) {
+        auto* base = static_cast<uint8_t*>(workspace);
+        SortBuffers buf;
+        for (int i = 0; i < 2; ++i) {
+            buf.keys[i] = reinterpret_cast<uint32_t*>(base + (2 * i) * need.list);
+            buf.values[i] = reinterpret_cast<uint32_t*>(base + (2 * i + 1) * need.list);
+        }
+        p.ends = reinterpret_cast<float*>(base + 4 * need.list);
+        const SortPlan s = sortPlan(tokens, vocab);
+        p.keys = buf.keys[(s.passes - 1) & 1];
+        p.values = buf.values[(s.passes - 1) & 1];
+        const size_t smem = static_cast<size_t>(kSortWarps + 2) * (1u << s.bits) * 4;
+        BFB_CUDA(cudaFuncSetAttribute(sortTokensKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(static_cast<unsigned>(s.cluster));
+        cfg.blockDim = dim3(kSortThreads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = stream;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = static_cast<unsigned>(s.cluster);
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        BFB_CUDA(cudaLaunchKernelEx(&cfg, sortTokensKernel, ids, buf, tokens, vocab, s.passes, s.bits, s.cluster));
+        noteLaunch();
+    }
+    using bf = __nv_bfloat16;
+    if (doutDtype == BFB_F32) {
+        if (dtableDtype == BFB_F32) reduceAnyPack<float, float>(p, stream);
+        else reduceAnyPack<float, bf>(p, stream);
+    } else {
+        if (dtableDtype == BFB_F32) reduceAnyPack<bf, float>(p, stream);
+        else reduceAnyPack<bf, bf>(p, stream);
+    }
+}
+
+}  // namespace bfb

@@ -207,6 +207,36 @@ void ceDxTensorCore(const LinearCeArgs& a, int64_t firstColumn, int64_t columns,
                     int64_t ldOut, const float* addend, int64_t ldAddend, cudaStream_t stream);
 void ceDwTensorCore(const LinearCeArgs& a, int64_t firstColumn, int64_t columns, const void* dz, int64_t ldDz, cudaStream_t stream);
 
+// Embedding lookup with a scale and the gradient of the table by sorted tokens (embed_grad.cu).
+void embedScaled(const float* ids, const void* table, int tableDtype, void* out, int outDtype, int64_t ldOut, int64_t tokens, int64_t vocab,
+                 int64_t dim, float scale, int* oobCount, cudaStream_t stream);
+size_t embedScaledBackwardWorkspaceBytes(int64_t tokens, int64_t vocab, int64_t dim);
+void embedScaledBackward(const float* ids, const void* dout, int doutDtype, int64_t ldDout, void* dtable, int dtableDtype, int64_t tokens,
+                         int64_t vocab, int64_t dim, float scale, bool accumulate, void* workspace, size_t workspaceBytes,
+                         cudaStream_t stream);
+
+// Distillation from a teacher's top logits, loss and gradient (distill.cu).
+struct DistillArgs {
+    const void* logits = nullptr;      // [rows, vocab], row pitch ldLogits
+    int dtype = 0;
+    int64_t ldLogits = 0;
+    const float* ids = nullptr;        // [rows, k] class indices held in float32; negative = no entry
+    const void* teacher = nullptr;     // [rows, k] the teacher's logits there
+    int teacherDtype = 0;
+    int64_t rows = 0, vocab = 0, k = 0;
+    float tau = 1.0f;
+    const float* gradLoss = nullptr;   // [rows] or null (1)
+    const float* dGradScale = nullptr; // one word on the device or null (1)
+    float gradScale = 1.0f;
+    float* loss = nullptr;             // [rows] or null
+    float* lse = nullptr;              // [rows] or null
+    void* grad = nullptr;              // [rows, vocab], row pitch ldGrad, or null; may be the logits
+    int gradDtype = 0;
+    int64_t ldGrad = 0;
+    int* oobCount = nullptr;
+};
+void distillTopk(const DistillArgs& args, cudaStream_t stream);
+
 // Tensor-core kernels (gemm_tc.cu / attention_tc.cu); callers have checked eligibility.
 void gemmTensorCore(const GemmArgs& args, cudaStream_t stream);
 // CTA-pair variant (cta_group::2, 256 x 256 tiles); B must be [N,K].

@@ -349,6 +349,47 @@ bfb_status bfb_linear_cross_entropy_bwd(const void* d_x, int64_t ld_x, const voi
                                         int64_t vocab, int64_t dim, void* d_workspace, size_t workspace_bytes,
                                         int32_t* d_status, void* stream);
 
+/* ---- embedding lookup with a scale, and the gradient of the table -------------------------------
+ * out[t, :] = scale * table[lround(ids[t]), :]. Beside bfb_embed_pos: tables and outputs in BFB_F32 or BFB_BF16, the scaled
+ * embeddings some decoders use, an output pitch (ld_out elements). Rows whose id is outside [0, vocab) or not finite are
+ * zero and counted in *d_oob_count, as there. */
+bfb_status bfb_embed_scaled(const float* d_ids, const void* d_table, int32_t table_dtype, void* d_out, int32_t out_dtype,
+                            int64_t ld_out, int64_t tokens, int64_t vocab, int64_t dim, float scale, int32_t* d_oob_count,
+                            void* stream);
+/* d_dtable[v, :] = scale * (sum over the tokens t with id v of d_dout[t, :]), dense [vocab, dim] in BFB_F32 or BFB_BF16.
+ * Replaces embeddingLookupBackward (src/backend/cuda/autodiff.cu:25-278), whose atomic scatter-add gives other bits on every
+ * run: here the tokens are sorted by id first and each row is summed in fp32 in the order of its tokens. Every row is written
+ * (zero where no token names it); with accumulate != 0 the sums are added to what is there instead, and other rows stay
+ * as they are: the second half of a tied table's gradient, or another micro-batch. Tokens whose id names no row add nothing.
+ * The workspace (bfb_embed_scaled_bwd_workspace bytes, 256-byte aligned) is the caller's, as for the linear cross entropy. */
+bfb_status bfb_embed_scaled_bwd_workspace(int64_t tokens, int64_t vocab, int64_t dim, size_t* bytes);
+bfb_status bfb_embed_scaled_bwd(const float* d_ids, const void* d_dout, int32_t dout_dtype, int64_t ld_dout, void* d_dtable,
+                                int32_t dtable_dtype, int64_t tokens, int64_t vocab, int64_t dim, float scale,
+                                int32_t accumulate, void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* ---- distillation from a teacher's top logits ----------------------------------------------------
+ * Loss and gradient in one pass over the student's logits, as the reference's loss kernels give both at once
+ * (src/backend/cuda/loss.cu:16-200); with k = 1 it is their sparse softmax cross entropy on stored logits.
+ *   q = softmax(d_teacher_logits[t, :] / temperature) over the k listed entries
+ *   p = softmax(d_logits[t, :] / temperature) over the vocabulary
+ *   d_loss[t] = temperature^2 * sum_k q_k (log q_k - log p_{id_k})
+ *   d_dlogits[t, j] = g_t * temperature * (p_j - sum of q_k over the entries with id_k = j)
+ * with g_t = grad_scale * *d_grad_scale * d_grad_loss[t] (device operands may be NULL, standing for 1).
+ *  d_logits [rows, vocab] BFB_F32 or BFB_BF16, pitch ld_logits, any alignment; d_teacher_ids [rows, k] float32 holding
+ *  integers; d_teacher_logits [rows, k] BFB_F32 or BFB_BF16; 1 <= k <= 1024. An entry with a negative id or a teacher
+ *  logit of -inf is left out; one at or above vocab, or not finite, too, and is counted in *d_oob_count (optional). An id
+ *  may be listed more than once. A row without an entry has loss 0 and gradient 0. Student logits of -inf have
+ *  probability 0 (an entry there with q > 0 makes the loss +inf); a row of nothing but -inf, or with NaN or +inf, has loss
+ *  and gradient NaN.
+ *  d_loss, d_lse (log sum exp of d_logits / temperature) and d_dlogits (grad_dtype BFB_F32 or BFB_BF16, pitch
+ *  ld_dlogits) may each be NULL. d_dlogits may be d_logits itself (same format and pitch), but not overlap it otherwise.
+ *  Everything is summed in fp32 in an order that depends on the sizes and on where a row starts in a 16-byte line only. */
+bfb_status bfb_distill_topk(const void* d_logits, int32_t dtype, int64_t ld_logits, const float* d_teacher_ids,
+                            const void* d_teacher_logits, int32_t teacher_dtype, int64_t k, float temperature,
+                            const float* d_grad_loss, const float* d_grad_scale, float grad_scale, float* d_loss,
+                            float* d_lse, void* d_dlogits, int32_t grad_dtype, int64_t ld_dlogits, int64_t rows,
+                            int64_t vocab, int32_t* d_oob_count, void* stream);
+
 /* ---- model: the IR executor's device side ------------------------------------------------------
  * Replaces cuda::Model (src/backend/cuda/model.cu:139-306: constructor, forward, parameters),
  * cuda::Executor::run / makeSyntheticInput (src/backend/cuda/executor.cu:26-132) and

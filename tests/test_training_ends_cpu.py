@@ -54,3 +54,51 @@ def test_linear_cross_entropy_with_nothing_to_do(bfb):
     assert bfb.lib().bfb_linear_cross_entropy_bwd(*args.values()) == bfb.OK
     args = {**FWD, "tokens": 0, "x": None, "labels": None, "lse": None, "ws": None, "ws_bytes": 0}
     assert bfb.lib().bfb_linear_cross_entropy_fwd(*args.values()) == bfb.OK
+
+
+# ---- scaled embedding -------------------------------------------------------------------------------------------
+
+LOOKUP = dict(ids=4096, table=4096, table_dtype=0, out=4096, out_dtype=0, ld_out=8, tokens=4, vocab=10, dim=8, scale=1.0, oob=None, stream=None)
+SCATTER = dict(ids=4096, dout=4096, dout_dtype=0, ld_dout=8, dtable=4096, dtable_dtype=0, tokens=4, vocab=10, dim=8, scale=1.0, accumulate=0,
+               ws=4096, ws_bytes=1 << 20, stream=None)
+
+
+@pytest.mark.parametrize("change", [dict(ids=None), dict(table=None), dict(out=None), dict(table_dtype=2), dict(out_dtype=2), dict(ld_out=7),
+                                    dict(tokens=-1), dict(vocab=0), dict(dim=0), dict(vocab=(1 << 24) + 1), dict(tokens=1 << 31)])
+def test_embed_scaled_refuses(bfb, change):
+    assert bfb.lib().bfb_embed_scaled(*{**LOOKUP, **change}.values()) == bfb.INVALID_ARGUMENT
+    assert b"embed_scaled" in bfb.lib().bfb_last_error()
+
+
+@pytest.mark.parametrize("change", [dict(ids=None), dict(dout=None), dict(dtable=None), dict(dout_dtype=2), dict(dtable_dtype=2), dict(ld_dout=7),
+                                    dict(tokens=-1), dict(vocab=0), dict(dim=0), dict(ws=None), dict(ws=4104), dict(ws_bytes=100)])
+def test_embed_scaled_backward_refuses(bfb, change):
+    assert bfb.lib().bfb_embed_scaled_bwd(*{**SCATTER, **change}.values()) == bfb.INVALID_ARGUMENT
+    assert b"embed_scaled" in bfb.lib().bfb_last_error()
+
+
+def test_embed_scaled_sizes_and_nothing_to_do(bfb):
+    st, n = size(bfb, "bfb_embed_scaled_bwd_workspace", 65536, 32000, 2048)
+    assert st == bfb.OK and 4 * 65536 * 4 <= n <= 4 * 65536 * 4 + 65536 // 8 * 2048 * 8
+    assert size(bfb, "bfb_embed_scaled_bwd_workspace", 4, 0, 8) == (bfb.INVALID_ARGUMENT, 0)
+    assert bfb.lib().bfb_embed_scaled(*{**LOOKUP, "tokens": 0, "ids": None}.values()) == bfb.OK
+    assert bfb.lib().bfb_embed_scaled_bwd(*{**SCATTER, "tokens": 0, "ids": None, "dout": None, "ws": None, "accumulate": 1}.values()) == bfb.OK
+
+
+# ---- distillation -----------------------------------------------------------------------------------------------
+
+DISTILL = dict(z=4096, dtype=0, ld=10, ids=4096, teacher=4096, teacher_dtype=0, k=3, tau=1.0, grad_loss=None, d_scale=None, scale=1.0, loss=4096,
+               lse=4096, grad=8192, grad_dtype=0, ld_grad=10, rows=4, vocab=10, oob=None, stream=None)
+
+
+@pytest.mark.parametrize("change", [dict(z=None), dict(ids=None), dict(teacher=None), dict(dtype=2), dict(teacher_dtype=2), dict(grad_dtype=2),
+                                    dict(ld=9), dict(ld_grad=9), dict(k=0), dict(k=1025), dict(tau=0.0), dict(tau=-1.0), dict(tau=float("nan")),
+                                    dict(tau=float("inf")), dict(rows=-1), dict(vocab=0), dict(vocab=(1 << 24) + 1, ld=1 << 25, ld_grad=1 << 25),
+                                    dict(grad=4096, grad_dtype=1), dict(grad=4096, ld_grad=11)])
+def test_distill_refuses(bfb, change):
+    assert bfb.lib().bfb_distill_topk(*{**DISTILL, **change}.values()) == bfb.INVALID_ARGUMENT
+    assert b"distill_topk" in bfb.lib().bfb_last_error()
+
+
+def test_distill_with_nothing_to_do(bfb):
+    assert bfb.lib().bfb_distill_topk(*{**DISTILL, "rows": 0, "z": None}.values()) == bfb.OK
