@@ -63,29 +63,39 @@ struct alignas(sizeof(T) * kN < 16 ? sizeof(T) * kN : 16) Pack {
 
 // ---- lookup --------------------------------------------------------------------------------------------------
 
-// blockDim.x threads across a row's packs, blockDim.y tokens per block.
+// blockDim.x threads across a row's packs, blockDim.y groups of kTokens tokens: the ids, then the rows of a group are all in
+// flight at once.
+constexpr int kTokens = 4;
+
 template <typename TIn, typename TOut, int kN>
 __global__ void __launch_bounds__(256)
 embedScaledKernel(const float* __restrict__ ids, const TIn* __restrict__ table, TOut* __restrict__ out, int64_t ldOut, int64_t tokens,
                   int64_t vocab, int64_t dim, float scale, int* oobCount) {
     const int64_t packs = dim / kN;
-    for (int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y; t < tokens; t += static_cast<int64_t>(gridDim.x) * blockDim.y) {
-        const uint32_t id = tokenRow(ids[t], vocab);
-        const bool ok = id < vocab;
-        if (!ok && threadIdx.x == 0 && oobCount != nullptr) atomicAdd(oobCount, 1);
-        const auto* src = reinterpret_cast<const Pack<TIn, kN>*>(table + static_cast<int64_t>(ok ? id : 0) * dim);
-        auto* dst = reinterpret_cast<Pack<TOut, kN>*>(out + t * ldOut);
+    const int64_t groups = (tokens + kTokens - 1) / kTokens;
+    for (int64_t group = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y; group < groups; group += static_cast<int64_t>(gridDim.x) * blockDim.y) {
+        const int64_t t0 = group * kTokens;
+        uint32_t id[kTokens];
+#pragma unroll
+        for (int u = 0; u < kTokens; ++u) id[u] = t0 + u < tokens ? tokenRow(__ldg(ids + t0 + u), vocab) : static_cast<uint32_t>(vocab);
+        if (threadIdx.x == 0 && oobCount != nullptr) {
+#pragma unroll
+            for (int u = 0; u < kTokens; ++u)
+                if (t0 + u < tokens && id[u] >= vocab) atomicAdd(oobCount, 1);
+        }
         for (int64_t i = threadIdx.x; i < packs; i += blockDim.x) {
-            Pack<TOut, kN> r;
-            if (ok) {
-                const Pack<TIn, kN> v = src[i];
+            Pack<TIn, kN> v[kTokens];
 #pragma unroll
-                for (int j = 0; j < kN; ++j) r.v[j] = fromFloat<TOut>(toFloat(v.v[j]) * scale);
-            } else {
+            for (int u = 0; u < kTokens; ++u)
+                if (id[u] < vocab) v[u] = reinterpret_cast<const Pack<TIn, kN>*>(table + static_cast<int64_t>(id[u]) * dim)[i];
 #pragma unroll
-                for (int j = 0; j < kN; ++j) r.v[j] = fromFloat<TOut>(0.0f);
+            for (int u = 0; u < kTokens; ++u) {
+                if (t0 + u >= tokens) break;
+                Pack<TOut, kN> r;
+#pragma unroll
+                for (int j = 0; j < kN; ++j) r.v[j] = fromFloat<TOut>(id[u] < vocab ? toFloat(v[u].v[j]) * scale : 0.0f);
+                reinterpret_cast<Pack<TOut, kN>*>(out + (t0 + u) * ldOut)[i] = r;
             }
-            dst[i] = r;
         }
     }
 }
@@ -99,9 +109,11 @@ struct SortBuffers {
 
 // Stable radix sort of (row, position) pairs, `passes` digits of `bits` bits. The cluster's blocks, their warps and a
 // warp's batches of 32 take consecutive stretches of the list; a pair's place is: all smaller digits, the same digit in
-// stretches before its own, the same digit before it in its batch. Rows that name no id (vocab) end up last.
+// stretches before its own, the same digit before it in its batch. Rows that name no id (vocab) end up last. `occurs` gets a
+// bit for every row that is named.
 __global__ void __launch_bounds__(kSortThreads, 1)
-sortTokensKernel(const float* __restrict__ ids, SortBuffers buf, int64_t count, int64_t vocab, int passes, int bits, int cluster) {
+sortTokensKernel(const float* __restrict__ ids, SortBuffers buf, uint32_t* __restrict__ occurs, int64_t count, int64_t vocab, int passes, int bits,
+                 int cluster) {
     extern __shared__ uint32_t counts[];   // [kSortWarps][bins], then [bins] totals of this block, [bins] bases
     const int bins = 1 << bits;
     uint32_t* blockTotal = counts + kSortWarps * bins;
@@ -113,25 +125,46 @@ sortTokensKernel(const float* __restrict__ ids, SortBuffers buf, int64_t count, 
     const int64_t begin = min(count, (static_cast<int64_t>(rank) * kSortWarps + warp) * perWarp);
     const int64_t end = min(count, begin + perWarp);
     uint32_t* mine = counts + warp * bins;
-
+    const int64_t all32 = static_cast<int64_t>(cluster) * kSortThreads, me = static_cast<int64_t>(rank) * kSortThreads + tid;
+    for (int64_t i = me; i < (vocab + 31) / 32; i += all32) occurs[i] = 0;
+    constexpr int kBatch = 8;   // loads in flight per lane
     for (int pass = 0; pass < passes; ++pass) {
         const int shift = pass * bits;
         const uint32_t* srcKeys = buf.keys[(pass & 1) ^ 1];
         const uint32_t* srcValues = buf.values[(pass & 1) ^ 1];
         uint32_t* dstKeys = buf.keys[pass & 1];
         uint32_t* dstValues = buf.values[pass & 1];
-        auto keyAt = [&](int64_t i) { return pass == 0 ? tokenRow(ids[i], vocab) : __ldcg(srcKeys + i); };
+        // the stretch's keys from i0 on, a batch per lane; all loads first, whatever lies behind the end reads the last one again
+        auto keysAt = [&](int64_t i0, uint32_t (&key)[kBatch]) {
+            uint32_t raw[kBatch];
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                const int64_t i = min(i0 + 32 * u + lane, end - 1);
+                raw[u] = pass == 0 ? __float_as_uint(__ldg(ids + i)) : __ldcg(srcKeys + i);
+            }
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) key[u] = pass == 0 ? tokenRow(__uint_as_float(raw[u]), vocab) : raw[u];
+        };
         for (int i = tid; i < kSortWarps * bins; i += kSortThreads) counts[i] = 0;
         __syncthreads();
-        for (int64_t i = begin + lane; i < end; i += 32) atomicAdd(&mine[(keyAt(i) >> shift) & (bins - 1)], 1u);
+        for (int64_t i0 = begin; i0 < end; i0 += 32 * kBatch) {
+            uint32_t key[kBatch];
+            keysAt(i0, key);
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u)
+                if (i0 + 32 * u + lane < end) atomicAdd(&mine[(key[u] >> shift) & (bins - 1)], 1u);
+        }
         __syncthreads();
         // per digit: what the block's earlier warps hold, and the block's total
         if (tid < bins) {
+            uint32_t held[kSortWarps];
+#pragma unroll
+            for (int w = 0; w < kSortWarps; ++w) held[w] = counts[w * bins + tid];
             uint32_t total = 0;
+#pragma unroll
             for (int w = 0; w < kSortWarps; ++w) {
-                const uint32_t n = counts[w * bins + tid];
                 counts[w * bins + tid] = total;
-                total += n;
+                total += held[w];
             }
             blockTotal[tid] = total;
         }
@@ -140,12 +173,19 @@ sortTokensKernel(const float* __restrict__ ids, SortBuffers buf, int64_t count, 
         // per digit: all blocks' totals, and those of the blocks before this one
         uint32_t all = 0, before = 0;
         if (tid < bins) {
-            for (int r = 0; r < cluster; ++r) {
-                uint32_t n;
-                const uint32_t from = mapa_cluster(smem_u32(&blockTotal[tid]), static_cast<uint32_t>(r));
-                asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(n) : "r"(from) : "memory");
-                all += n;
-                before += r < rank ? n : 0;
+            uint32_t theirs[kSortCluster];
+#pragma unroll
+            for (int r = 0; r < kSortCluster; ++r) {
+                theirs[r] = 0;
+                if (r < cluster) {
+                    const uint32_t from = mapa_cluster(smem_u32(&blockTotal[tid]), static_cast<uint32_t>(r));
+                    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(theirs[r]) : "r"(from) : "memory");
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < kSortCluster; ++r) {
+                all += theirs[r];
+                before += r < rank ? theirs[r] : 0;
             }
         }
         uint32_t scan = all;   // inclusive over the digits
@@ -161,29 +201,51 @@ sortTokensKernel(const float* __restrict__ ids, SortBuffers buf, int64_t count, 
         if (tid < bins) base[tid] = smaller + scan - all + before;
         __syncthreads();
         // places, 32 pairs at a time
-        for (int64_t i0 = begin; i0 < end; i0 += 32) {
-            const int64_t i = i0 + lane;
-            const bool live = i < end;
-            const uint32_t key = live ? keyAt(i) : 0;
-            const uint32_t value = live ? (pass == 0 ? static_cast<uint32_t>(i) : __ldcg(srcValues + i)) : 0;
-            const uint32_t digit = live ? (key >> shift) & (bins - 1) : 0xFFFFFFFFu;
-            const uint32_t same = __match_any_sync(0xFFFFFFFFu, digit);
-            if (live) {
-                const uint32_t earlier = __popc(same & ((1u << lane) - 1u));
-                const uint32_t at = base[digit] + mine[digit] + earlier;
-                if (at < count) {   // always, unless the ids change while the kernel runs
-                    dstKeys[at] = key;
-                    dstValues[at] = value;
-                }
+        for (int64_t i0 = begin; i0 < end; i0 += 32 * kBatch) {
+            uint32_t keys[kBatch], values[kBatch];
+            keysAt(i0, keys);
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                const int64_t i = min(i0 + 32 * u + lane, end - 1);
+                values[u] = pass == 0 ? static_cast<uint32_t>(i) : __ldcg(srcValues + i);
             }
-            __syncwarp();
-            if (live && lane == 31 - __clz(same)) mine[digit] += __popc(same);
-            __syncwarp();
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                if (i0 + 32 * u >= end) break;
+                const bool live = i0 + 32 * u + lane < end;
+                const uint32_t digit = live ? (keys[u] >> shift) & (bins - 1) : 0xFFFFFFFFu;
+                const uint32_t same = __match_any_sync(0xFFFFFFFFu, digit);
+                if (live) {
+                    const uint32_t earlier = __popc(same & ((1u << lane) - 1u));
+                    const uint32_t at = base[digit] + mine[digit] + earlier;
+                    if (at < count) {   // always, unless the ids change while the kernel runs
+                        dstKeys[at] = keys[u];
+                        dstValues[at] = values[u];
+                    }
+                }
+                __syncwarp();
+                if (live && lane == 31 - __clz(same)) mine[digit] += __popc(same);
+                __syncwarp();
+            }
         }
         // the next pass reads what other blocks wrote; and nobody leaves while its totals are being read
         __threadfence();
         if (cluster > 1) cluster_sync_all();
         else __syncthreads();
+    }
+    // where a run begins: its row occurs
+    const uint32_t* sorted = buf.keys[(passes - 1) & 1];
+    for (int64_t i0 = me; i0 < count; i0 += all32 * 4) {
+        uint32_t key[4], before[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int64_t i = i0 + u * all32;
+            key[u] = i < count ? __ldcg(sorted + i) : static_cast<uint32_t>(vocab);
+            before[u] = i > 0 && i < count ? __ldcg(sorted + i - 1) : 0xFFFFFFFFu;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (key[u] < vocab && key[u] != before[u]) atomicOr(occurs + (key[u] >> 5), 1u << (key[u] & 31));
     }
 }
 
@@ -192,6 +254,7 @@ sortTokensKernel(const float* __restrict__ ids, SortBuffers buf, int64_t count, 
 struct ReduceParams {
     const uint32_t* keys;      // sorted rows
     const uint32_t* values;    // token positions
+    const uint32_t* occurs;    // a bit for every row that is named (null: none is)
     int64_t count;             // entries, those that name no row last
     int64_t vocab, dim;
     const void* dout;
@@ -298,36 +361,22 @@ embedReduceKernel(const ReduceParams p) {
         return;
     }
     // ---- rows that do not occur: a block looks after kZeroRows neighbouring rows
-    __shared__ uint32_t seen[kZeroRows / 32];
     const int64_t row0 = (blockIdx.x - reduceBlocks) * kZeroRows;
     const int rows = static_cast<int>(min(static_cast<int64_t>(kZeroRows), p.vocab - row0));
-    if (tid < kZeroRows / 32) seen[tid] = 0;
-    __syncthreads();
-    // first sorted entry at or above row0: every warp narrows the range to a 33rd per step
-    int64_t low = 0, high = p.count;
-    while (low < high) {
-        const int64_t probe = low + (high - low) * (tid & 31) / 32;
-        const int below = __popc(__ballot_sync(0xFFFFFFFFu, p.keys[probe] < row0));   // the probes ascend
-        const int64_t next = low + (high - low) * below / 32;                         // first probe that is not below (or high)
-        const int64_t before = low + (high - low) * (below - 1) / 32;
-        if (below > 0) low = before + 1;
-        high = below == 0 ? low : next;
-    }
-    for (int64_t i = low + tid;; i += blockDim.x) {
-        const uint32_t key = i < p.count ? p.keys[i] : static_cast<uint32_t>(p.vocab);
-        const bool inside = key < static_cast<uint64_t>(row0) + rows && key < p.vocab;
-        if (inside) atomicOr(&seen[(key - row0) >> 5], 1u << ((key - row0) & 31));
-        if (__syncthreads_and(inside) == 0) break;
-    }
+    uint32_t seen[kZeroRows / 32];
+#pragma unroll
+    for (int w = 0; w < kZeroRows / 32; ++w) seen[w] = p.occurs != nullptr && row0 + w * 32 < p.vocab ? p.occurs[row0 / 32 + w] : 0;
+    auto occurs = [&](int r) { return ((r < 32 ? seen[0] : seen[1]) >> (r & 31)) & 1u; };
+    static_assert(kZeroRows == 64, "two words of the map per block");
     TOut* table = static_cast<TOut*>(p.dtable);
     int r = 0;
     while (r < rows) {
-        if ((seen[r >> 5] >> (r & 31)) & 1u) {
+        if (occurs(r)) {
             ++r;
             continue;
         }
         int to = r + 1;   // a stretch of rows without a token is one stretch of memory
-        while (to < rows && !((seen[to >> 5] >> (to & 31)) & 1u)) ++to;
+        while (to < rows && !occurs(to)) ++to;
         char* from = reinterpret_cast<char*>(table + (row0 + r) * p.dim);
         const int64_t bytes = static_cast<int64_t>(to - r) * p.dim * static_cast<int64_t>(sizeof(TOut));
         const int64_t head = min(bytes, static_cast<int64_t>((16 - reinterpret_cast<uintptr_t>(from) % 16) % 16));
@@ -343,7 +392,7 @@ embedReduceKernel(const ReduceParams p) {
 // ---- 3. runs that cross the borders of pieces --------------------------------------------------------------------
 
 // A piece whose last run goes on, and did not begin before the piece, starts a chain: its own part, then the first parts of
-// the pieces behind it that begin with the same row. One column per thread, parts added in order, eight in flight.
+// the pieces behind it that begin with the same row. One column per thread, parts added in order.
 template <typename TOut>
 __global__ void __launch_bounds__(256)
 embedJoinKernel(const ReduceParams p) {
@@ -354,18 +403,31 @@ embedJoinKernel(const ReduceParams p) {
     if (first == key && earlier == key) return;           // the chain started earlier
     const int64_t col = static_cast<int64_t>(blockIdx.y) * blockDim.x + threadIdx.x;
     if (col >= p.dim) return;
-    constexpr int kAhead = 8;
+    // Most chains end with the next piece. A long one goes on in batches: the keys that tell how far it goes and the parts
+    // themselves are fetched at once (all loads first; behind the last piece they read that one again).
+    constexpr int kAhead = 16;
     float sum = p.ends[(piece * 2 + 1) * p.dim + col];
-    for (int64_t q = piece + 1;; q += kAhead) {
-        bool in[kAhead];
-        float part[kAhead];
+    const float second = p.ends[(piece + 1) * 2 * p.dim + col];
+    const uint32_t third = p.keys[min(piece + 2, p.pieces - 1) * p.piece];
+    sum += second;
+    if (piece + 2 < p.pieces && third == key) {
+        for (int64_t q = piece + 2;; q += kAhead) {
+            float part[kAhead];
+            uint32_t keys[kAhead];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) in[u] = q + u < p.pieces && p.keys[(q + u) * p.piece] == key;
+            for (int u = 0; u < kAhead; ++u) {
+                const int64_t at = min(q + u, p.pieces - 1);
+                keys[u] = p.keys[at * p.piece];
+                part[u] = p.ends[at * 2 * p.dim + col];
+            }
+            bool more = true;
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) part[u] = in[u] ? p.ends[(q + u) * 2 * p.dim + col] : 0.0f;
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) sum += part[u];
-        if (!in[kAhead - 1]) break;
+            for (int u = 0; u < kAhead; ++u) {
+                more = more && q + u < p.pieces && keys[u] == key;
+                sum += more ? part[u] : 0.0f;
+            }
+            if (!more) break;
+        }
     }
     const float acc[1] = {sum};
     storeRow<TOut, 1>(static_cast<TOut*>(p.dtable) + static_cast<int64_t>(key) * p.dim, col, acc, p.scale, p.accumulate != 0);
@@ -380,18 +442,18 @@ SortPlan sortPlan(int64_t tokens, int64_t vocab) {
     SortPlan s;
     s.passes = (width + kMaxDigitBits - 1) / kMaxDigitBits;
     s.bits = (width + s.passes - 1) / s.passes;
-    s.cluster = tokens <= 4096 ? 1 : kSortCluster;
+    s.cluster = tokens <= 8192 ? 1 : kSortCluster;   // a block alone needs no cluster barriers and no fences beyond its SM
     return s;
 }
 
 struct EmbedWorkspace {
-    size_t list, ends, total;
+    size_t list, ends, map, total;
     int piece;
     int64_t pieces;
 };
 // Entries per piece: as many as leave eight blocks for each of 148 SMs (the ends of a piece cost two rows of fp32, so long
 // pieces move less), between 8 and 128.
-EmbedWorkspace embedWorkspace(int64_t tokens, int64_t dim) {
+EmbedWorkspace embedWorkspace(int64_t tokens, int64_t vocab, int64_t dim) {
     EmbedWorkspace w;
     const int64_t share = tokens * ((dim + 1023) / 1024) / (148 * 8);
     w.piece = 8;
@@ -399,7 +461,8 @@ EmbedWorkspace embedWorkspace(int64_t tokens, int64_t dim) {
     w.pieces = (tokens + w.piece - 1) / w.piece;
     w.list = static_cast<size_t>(roundUp(std::max<int64_t>(tokens, 1) * 4, 256));
     w.ends = static_cast<size_t>(roundUp(w.pieces * 2 * dim * 4, 256));
-    w.total = 4 * w.list + w.ends;
+    w.map = static_cast<size_t>(roundUp((vocab + 31) / 32 * 4, 256));
+    w.total = 4 * w.list + w.ends + w.map;
     return w;
 }
 
@@ -437,7 +500,7 @@ void launchLookup(const float* ids, const void* table, void* out, int64_t ldOut,
     const int64_t packs = wide ? dim / kWide : dim;
     const int across = static_cast<int>(std::min<int64_t>(256, roundUp(packs, 32)));
     const dim3 block(across, 256 / across);
-    const int64_t blocks = (tokens + block.y - 1) / block.y;
+    const int64_t blocks = (tokens + static_cast<int64_t>(block.y) * kTokens - 1) / (static_cast<int64_t>(block.y) * kTokens);
     const int grid = static_cast<int>(std::min<int64_t>(blocks, static_cast<int64_t>(smCount()) * 32));
     const auto* t = static_cast<const TIn*>(table);
     auto* o = static_cast<TOut*>(out);
@@ -474,7 +537,7 @@ void embedScaled(const float* ids, const void* table, int tableDtype, void* out,
 
 size_t embedScaledBackwardWorkspaceBytes(int64_t tokens, int64_t vocab, int64_t dim) {
     checkSizes(tokens, vocab, dim);
-    return embedWorkspace(tokens, dim).total;
+    return embedWorkspace(tokens, vocab, dim).total;
 }
 
 void embedScaledBackward(const float* ids, const void* dout, int doutDtype, int64_t ldDout, void* dtable, int dtableDtype, int64_t tokens,
@@ -486,7 +549,7 @@ void embedScaledBackward(const float* ids, const void* dout, int doutDtype, int6
     require(ldDout >= dim, "embed_scaled_bwd: row pitch smaller than dim");
     require(dtable != nullptr, "embed_scaled_bwd: null pointer");
     if (tokens > 0) require(ids != nullptr && dout != nullptr, "embed_scaled_bwd: null pointer");
-    const EmbedWorkspace need = embedWorkspace(tokens, dim);
+    const EmbedWorkspace need = embedWorkspace(tokens, vocab, dim);
     require(tokens == 0 || (workspace != nullptr && workspaceBytes >= need.total && reinterpret_cast<uintptr_t>(workspace) % 256 == 0),
             "embed_scaled_bwd: the workspace is missing, too small (bfb_embed_scaled_bwd_workspace) or not 256-byte aligned");
     ReduceParams p{};
@@ -508,6 +571,8 @@ void embedScaledBackward(const float* ids, const void* dout, int doutDtype, int6
             buf.values[i] = reinterpret_cast<uint32_t*>(base + (2 * i + 1) * need.list);
         }
         p.ends = reinterpret_cast<float*>(base + 4 * need.list);
+        auto* occurs = reinterpret_cast<uint32_t*>(base + 4 * need.list + need.ends);
+        p.occurs = occurs;
         const SortPlan s = sortPlan(tokens, vocab);
         p.keys = buf.keys[(s.passes - 1) & 1];
         p.values = buf.values[(s.passes - 1) & 1];
@@ -525,7 +590,7 @@ void embedScaledBackward(const float* ids, const void* dout, int doutDtype, int6
         attr[0].val.clusterDim.z = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        BFB_CUDA(cudaLaunchKernelEx(&cfg, sortTokensKernel, ids, buf, tokens, vocab, s.passes, s.bits, s.cluster));
+        BFB_CUDA(cudaLaunchKernelEx(&cfg, sortTokensKernel, ids, buf, occurs, tokens, vocab, s.passes, s.bits, s.cluster));
         noteLaunch();
     }
     using bf = __nv_bfloat16;
