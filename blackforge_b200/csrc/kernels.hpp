@@ -203,9 +203,13 @@ void linearCeBackward(const LinearCeArgs& args, cudaStream_t stream);
 void ceStatsTensorCore(const LinearCeArgs& a, float2* partials, float* labelLogit, cudaStream_t stream);
 void ceDzTensorCore(const LinearCeArgs& a, int64_t firstColumn, int64_t columns, void* dz, int64_t ldDz, float* biasPartials,
                     cudaStream_t stream);
+// Parts the reduction of an [m, n] gradient product over k is split into (1: no split); with more than one, the products
+// write fp32 parts [splits][m][ldOut].
+int ceSplits(int64_t m, int64_t n, int64_t k);
 void ceDxTensorCore(const LinearCeArgs& a, int64_t firstColumn, int64_t columns, const void* dz, int64_t ldDz, void* out, int outDtype,
-                    int64_t ldOut, const float* addend, int64_t ldAddend, cudaStream_t stream);
-void ceDwTensorCore(const LinearCeArgs& a, int64_t firstColumn, int64_t columns, const void* dz, int64_t ldDz, cudaStream_t stream);
+                    int64_t ldOut, const float* addend, int64_t ldAddend, int splits, cudaStream_t stream);
+void ceDwTensorCore(const LinearCeArgs& a, int64_t columns, const void* dz, int64_t ldDz, void* out, int outDtype, int64_t ldOut, int splits,
+                    cudaStream_t stream);
 
 // Embedding lookup with a scale and the gradient of the table by sorted tokens (embed_grad.cu).
 void embedScaled(const float* ids, const void* table, int tableDtype, void* out, int outDtype, int64_t ldOut, int64_t tokens, int64_t vocab,

@@ -13,7 +13,8 @@
 //
 // bf16 operands on 16-byte rows run on the tensor cores (linear_ce_tc.cu). fp32 operands, where products in fp32 are
 // the contract, and bf16 rows that TMA cannot read run on the CUDA-core kernel below: 64 x 64 tiles, 4 x 4 per thread,
-// the same two epilogues, dz kept in fp32.
+// the same two epilogues, dz kept in fp32. A gradient product with few tiles and a long reduction is split over it on both
+// routes; the parts are added in order.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -36,7 +37,7 @@ inline bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 1
 
 // ---- CUDA-core products -----------------------------------------------------------------------------------
 
-constexpr int kTile = 64, kDepth = 16;
+constexpr int kTile = 64, kDepth = 32;
 
 template <typename T>
 __device__ __forceinline__ float ceLoad(const void* p, int64_t i);
@@ -69,39 +70,57 @@ struct CeSimtArgs {
     int64_t ldOut;
     const float* addend;        // fp32 [m][ldAddend] or null
     int64_t ldAddend;
+    int64_t kPerSplit;          // part of the reduction per blockIdx.y; parts go to [split][m][ldOut]
 };
 
 enum { kSimtStats = 0, kSimtDz = 1, kSimtGrad = 2 };
 
+// The next slice of the operands is on its way to registers while this one is used: at these sizes a slice costs a trip to
+// memory, not its arithmetic.
 template <int kMode, typename TA, typename TB, typename TC>
-__global__ void __launch_bounds__(256) ceSimtKernel(const CeSimtArgs p) {
-    __shared__ float sa[kDepth][kTile + 1];
-    __shared__ float sb[kDepth][kTile + 1];
+__global__ void __launch_bounds__(256, 2) ceSimtKernel(const CeSimtArgs p) {
+    __shared__ alignas(16) float sa[kDepth][kTile + 4];
+    __shared__ alignas(16) float sb[kDepth][kTile + 4];
     __shared__ float2 rowStat[kTile][16];
+    constexpr int kEach = kTile * kDepth / 256;
     const int tid = threadIdx.x;
     const int tx = tid & 15, ty = tid >> 4;
     const int64_t tilesN = (p.n + kTile - 1) / kTile;
     const int64_t tilesM = (p.m + kTile - 1) / kTile;
+    const int64_t kBegin = static_cast<int64_t>(blockIdx.y) * p.kPerSplit, kEnd = min(p.k, kBegin + p.kPerSplit);
+    const bool aAlong = p.aDepth == 1, bAlong = p.bDepth == 1;   // neighbouring threads go where memory is contiguous
     for (int64_t tile = blockIdx.x; tile < tilesM * tilesN; tile += gridDim.x) {
         const int64_t m0 = (tile / tilesN) * kTile, n0 = (tile % tilesN) * kTile;
         float acc[4][4] = {};
-        for (int64_t k0 = 0; k0 < p.k; k0 += kDepth) {
+        float ra[kEach], rb[kEach];
+        auto fetch = [&](int64_t k0) {
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) {
+                const int i = tid + e * 256;
+                const int r0 = aAlong ? i / kDepth : i % kTile, k1 = aAlong ? i % kDepth : i / kTile;
+                const int r2 = bAlong ? i / kDepth : i % kTile, k3 = bAlong ? i % kDepth : i / kTile;
+                ra[e] = m0 + r0 < p.m && k0 + k1 < kEnd ? ceLoad<TA>(p.a, (m0 + r0) * p.aRow + (k0 + k1) * p.aDepth) : 0.0f;
+                rb[e] = n0 + r2 < p.n && k0 + k3 < kEnd ? ceLoad<TB>(p.b, (n0 + r2) * p.bRow + (k0 + k3) * p.bDepth) : 0.0f;
+            }
+        };
+        fetch(kBegin);
+        for (int64_t k0 = kBegin; k0 < kEnd; k0 += kDepth) {
             __syncthreads();
-            for (int i = tid; i < kTile * kDepth; i += 256) {
-                // neighbouring threads along whichever direction is contiguous in memory
-                const int ra = p.aDepth == 1 ? i / kDepth : i % kTile, ka = p.aDepth == 1 ? i % kDepth : i / kTile;
-                const int rb = p.bDepth == 1 ? i / kDepth : i % kTile, kb = p.bDepth == 1 ? i % kDepth : i / kTile;
-                sa[ka][ra] = m0 + ra < p.m && k0 + ka < p.k ? ceLoad<TA>(p.a, (m0 + ra) * p.aRow + (k0 + ka) * p.aDepth) : 0.0f;
-                sb[kb][rb] = n0 + rb < p.n && k0 + kb < p.k ? ceLoad<TB>(p.b, (n0 + rb) * p.bRow + (k0 + kb) * p.bDepth) : 0.0f;
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) {
+                const int i = tid + e * 256;
+                if (aAlong) sa[i % kDepth][i / kDepth] = ra[e];
+                else sa[i / kTile][i % kTile] = ra[e];
+                if (bAlong) sb[i % kDepth][i / kDepth] = rb[e];
+                else sb[i / kTile][i % kTile] = rb[e];
             }
             __syncthreads();
+            if (k0 + kDepth < kEnd) fetch(k0 + kDepth);
 #pragma unroll
             for (int kk = 0; kk < kDepth; ++kk) {
-                float av[4], bv[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) av[i] = sa[kk][ty * 4 + i];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) bv[j] = sb[kk][tx * 4 + j];
+                const float4 a4 = *reinterpret_cast<const float4*>(&sa[kk][ty * 4]);
+                const float4 b4 = *reinterpret_cast<const float4*>(&sb[kk][tx * 4]);
+                const float av[4] = {a4.x, a4.y, a4.z, a4.w}, bv[4] = {b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -109,7 +128,7 @@ __global__ void __launch_bounds__(256) ceSimtKernel(const CeSimtArgs p) {
             }
         }
         if constexpr (kMode == kSimtGrad) {
-            TC* out = static_cast<TC*>(p.out);
+            TC* out = static_cast<TC*>(p.out) + static_cast<int64_t>(blockIdx.y) * p.m * p.ldOut;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int64_t row = m0 + ty * 4 + i;
@@ -173,33 +192,37 @@ __global__ void __launch_bounds__(256) ceSimtKernel(const CeSimtArgs p) {
 
 // ---- joining the pieces of the forward --------------------------------------------------------------------------
 
-// 32 rows per block, the parts of a row split over the block's eight warps and joined through shared memory.
-__global__ void __launch_bounds__(256)
+// 32 rows per block, the parts of a row split over the block's warps and joined through shared memory, in the same order on
+// every run. A warp's parts come in batches of four.
+__global__ void __launch_bounds__(1024)
 ceFinishKernel(const float2* __restrict__ partials, int64_t parts, const float* __restrict__ labelLogit, const float* __restrict__ labels,
                int64_t vocab, float* loss, float* lse, int64_t tokens, int* oobCount) {
-    __shared__ float2 joined[8][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __shared__ float2 joined[32][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const int64_t row = static_cast<int64_t>(blockIdx.x) * 32 + lane;
     float top = -INFINITY, sum = 0.0f;
+    auto join = [&](const float2& s) {
+        const float next = fmaxf(top, s.x);
+        const float at = next == -INFINITY ? 0.0f : next;
+        sum = sum * exp2f((top - at) * kLog2e) + s.y * exp2f((s.x - at) * kLog2e);
+        top = next;
+    };
     if (row < tokens) {
-        for (int64_t part = warp; part < parts; part += 8) {
-            const float2 s = partials[part * tokens + row];
-            const float next = fmaxf(top, s.x);
-            const float at = next == -INFINITY ? 0.0f : next;
-            sum = sum * exp2f((top - at) * kLog2e) + s.y * exp2f((s.x - at) * kLog2e);
-            top = next;
+        for (int64_t part = warp; part < parts; part += 4 * warps) {
+            float2 s[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int64_t at = part + u * warps;
+                s[u] = at < parts ? partials[at * tokens + row] : make_float2(-INFINITY, 0.0f);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) join(s[u]);
         }
     }
     joined[warp][lane] = make_float2(top, sum);
     __syncthreads();
     if (warp != 0 || row >= tokens) return;
-    for (int w = 1; w < 8; ++w) {
-        const float2 s = joined[w][lane];
-        const float next = fmaxf(top, s.x);
-        const float at = next == -INFINITY ? 0.0f : next;
-        sum = sum * exp2f((top - at) * kLog2e) + s.y * exp2f((s.x - at) * kLog2e);
-        top = next;
-    }
+    for (int w = 1; w < warps; ++w) join(joined[w][lane]);
     const float value = top + logf(sum);   // no column above -inf: -inf + log 0, a row without a distribution
     lse[row] = value;
     const float label = labels[row];
@@ -215,10 +238,20 @@ ceSummaryKernel(const float* __restrict__ loss, const float* __restrict__ labels
     __shared__ unsigned long long counts[32];
     double sum = 0.0;
     unsigned long long count = 0;
-    for (int64_t i = threadIdx.x; i < tokens; i += 1024) {
-        if (ceLabel(labels[i], vocab) >= 0) {
-            sum += loss[i];
-            ++count;
+    for (int64_t i0 = threadIdx.x; i0 < tokens; i0 += 8 * 1024) {
+        float label[8], value[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {   // all loads of a batch before its sums
+            const int64_t i = min(i0 + u * 1024, tokens - 1);
+            label[u] = labels[i];
+            value[u] = loss[i];
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            if (i0 + u * 1024 < tokens && ceLabel(label[u], vocab) >= 0) {
+                sum += value[u];
+                ++count;
+            }
         }
     }
 #pragma unroll
@@ -258,6 +291,37 @@ ceColumnSumKernel(const float* __restrict__ in, int64_t ld, int64_t rows, int64_
     out[col] = sum;
 }
 
+// out = sum of the parts of a split product, in order, + addend.
+template <typename TC>
+__global__ void __launch_bounds__(256)
+cePartSumKernel(const float* __restrict__ parts, int splits, int64_t rows, int64_t cols, const float* addend, int64_t ldAddend, TC* out,
+                int64_t ldOut) {
+    const int64_t total = rows * cols, step = static_cast<int64_t>(gridDim.x) * blockDim.x;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += step) {
+        const int64_t row = i / cols, col = i - row * cols;
+        float sum = parts[i];
+        for (int s0 = 1; s0 < splits; s0 += 4) {
+            float v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v[u] = s0 + u < splits ? parts[(s0 + u) * total + i] : 0.0f;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) sum += v[u];
+        }
+        if (addend != nullptr) sum += addend[row * ldAddend + col];
+        if constexpr (sizeof(TC) == 4) out[row * ldOut + col] = sum;
+        else out[row * ldOut + col] = __float2bfloat16_rn(sum);
+    }
+}
+
+void cePartSum(const float* parts, int splits, int64_t rows, int64_t cols, const float* addend, int64_t ldAddend, void* out, int outDtype,
+               int64_t ldOut, cudaStream_t stream) {
+    const int grid = static_cast<int>(std::min<int64_t>((rows * cols + 255) / 256, static_cast<int64_t>(smCount()) * 16));
+    if (outDtype == BFB_F32) cePartSumKernel<float><<<grid, 256, 0, stream>>>(parts, splits, rows, cols, addend, ldAddend, static_cast<float*>(out), ldOut);
+    else cePartSumKernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(parts, splits, rows, cols, addend, ldAddend, static_cast<__nv_bfloat16*>(out), ldOut);
+    BFB_LAUNCH_CHECK();
+    noteLaunch();
+}
+
 __global__ void ceZeroRowsKernel(void* out, int dtype, int64_t ld, int64_t rows, int64_t cols) {
     const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < rows * cols; i += step) {
@@ -284,6 +348,7 @@ CeSimtArgs simtOperands(const LinearCeArgs& a, int64_t firstColumn, int64_t colu
     p.m = a.tokens;
     p.n = columns;
     p.k = a.dim;
+    p.kPerSplit = a.dim;
     p.bias = a.bias == nullptr ? nullptr : a.bias + firstColumn;
     p.labels = a.labels;
     p.vocab = a.vocab;
@@ -299,9 +364,18 @@ struct CePlan {
     int64_t pieceColumns = 0;   // vocabulary columns per piece of the backward
     int64_t pieces = 0;
     int64_t ldDz = 0;
-    size_t forwardBytes = 0, dzBytes = 0, biasBytes = 0, dxBytes = 0;
-    size_t backwardBytes() const { return dzBytes + biasBytes + dxBytes; }
+    int splitsDx = 1, splitsDw = 1;
+    size_t forwardBytes = 0, dzBytes = 0, biasBytes = 0, dxBytes = 0, partBytes = 0;
+    size_t backwardBytes() const { return dzBytes + biasBytes + dxBytes + partBytes; }
 };
+
+// The CUDA-core products: parts of at least 64 until there are two blocks for each of 148 SMs.
+int simtSplits(int64_t m, int64_t n, int64_t k) {
+    const int64_t tiles = ((m + kTile - 1) / kTile) * ((n + kTile - 1) / kTile);
+    const int64_t want = std::max<int64_t>(1, std::min((2 * 148 + tiles - 1) / tiles, (k + 63) / 64));
+    const int64_t per = (k + want - 1) / want;
+    return static_cast<int>((k + per - 1) / per);
+}
 
 // The piece is as wide as its dz stays within 256 MiB, at least 4096 columns (narrower pieces make the dx product so
 // shallow that the fp32 sums it carries from piece to piece cost more than its MMAs), all pieces equally wide.
@@ -322,6 +396,11 @@ CePlan cePlan(int64_t tokens, int64_t vocab, int64_t dim, bool tensorCores) {
     p.dzBytes = static_cast<size_t>(roundUp(rows * p.ldDz * elem, 256));
     p.biasBytes = tensorCores ? static_cast<size_t>(roundUp((rows + 31) / 32 * p.ldDz * 4, 256)) : 0;
     p.dxBytes = p.pieces > 1 ? static_cast<size_t>(roundUp(rows * dim * 4, 256)) : 0;
+    // all pieces alike, the narrower last one too
+    p.splitsDx = tensorCores ? ceSplits(rows, dim, p.pieceColumns) : simtSplits(rows, dim, p.pieceColumns);
+    p.splitsDw = tensorCores ? ceSplits(p.pieceColumns, dim, rows) : simtSplits(p.pieceColumns, dim, rows);
+    const int64_t partsDx = p.splitsDx > 1 ? p.splitsDx * rows * dim : 0, partsDw = p.splitsDw > 1 ? p.splitsDw * p.pieceColumns * dim : 0;
+    p.partBytes = static_cast<size_t>(roundUp(std::max(partsDx, partsDw) * 4, 256));
     return p;
 }
 
@@ -386,7 +465,9 @@ void linearCeForward(const LinearCeArgs& a, cudaStream_t stream) {
             BFB_LAUNCH_CHECK();
             noteLaunch();
         }
-        ceFinishKernel<<<static_cast<unsigned>((a.tokens + 31) / 32), 256, 0, stream>>>(partials, plan.parts, labelLogit, a.labels, a.vocab,
+        // a warp of 32 rows for every four parts, up to 32 of them
+        const int finishThreads = static_cast<int>(std::min<int64_t>(32, (plan.parts + 3) / 4)) * 32;
+        ceFinishKernel<<<static_cast<unsigned>((a.tokens + 31) / 32), finishThreads, 0, stream>>>(partials, plan.parts, labelLogit, a.labels, a.vocab,
                                                                                       a.loss, a.lse, a.tokens, a.oobCount);
         BFB_LAUNCH_CHECK();
         noteLaunch();
@@ -422,6 +503,24 @@ void linearCeBackward(const LinearCeArgs& a, cudaStream_t stream) {
     void* dz = base;
     auto* biasPartials = reinterpret_cast<float*>(base + plan.dzBytes);
     auto* dxSum = reinterpret_cast<float*>(base + plan.dzBytes + plan.biasBytes);
+    auto* parts = reinterpret_cast<float*>(base + plan.dzBytes + plan.biasBytes + plan.dxBytes);
+    const bool f32 = a.dtype == BFB_F32;
+    auto simtProduct = [&](CeSimtArgs g, const void* b, bool bIsF32, int outDtype, int splits) {
+        g.b = b;
+        g.kPerSplit = (g.k + splits - 1) / splits;
+        const dim3 grid(simtGrid(g.m, g.n), static_cast<unsigned>((g.k + g.kPerSplit - 1) / g.kPerSplit));
+        if (bIsF32 && outDtype == BFB_F32) ceSimtKernel<kSimtGrad, float, float, float><<<grid, 256, 0, stream>>>(g);
+        else if (bIsF32) ceSimtKernel<kSimtGrad, float, float, __nv_bfloat16><<<grid, 256, 0, stream>>>(g);
+        else if (outDtype == BFB_F32) ceSimtKernel<kSimtGrad, float, __nv_bfloat16, float><<<grid, 256, 0, stream>>>(g);
+        else ceSimtKernel<kSimtGrad, float, __nv_bfloat16, __nv_bfloat16><<<grid, 256, 0, stream>>>(g);
+        BFB_LAUNCH_CHECK();
+        noteLaunch();
+        return static_cast<int>(grid.y);
+    };
+    auto partsOf = [](int64_t k, int splits, int64_t unit) {   // parts a product over k is really cut into
+        const int64_t stages = (k + unit - 1) / unit, per = (stages + splits - 1) / splits;
+        return static_cast<int>((stages + per - 1) / per);
+    };
     for (int64_t piece = 0; piece < plan.pieces; ++piece) {
         const int64_t first = piece * plan.pieceColumns;
         const int64_t columns = std::min(plan.pieceColumns, a.vocab - first);
@@ -431,10 +530,19 @@ void linearCeBackward(const LinearCeArgs& a, cudaStream_t stream) {
         void* dxOut = last ? a.dx : static_cast<void*>(dxSum);
         const int dxType = last ? a.gradDtype : BFB_F32;
         const int64_t ldDxOut = last ? a.ldDx : a.dim;
+        void* dwOut = a.dw == nullptr ? nullptr : static_cast<uint8_t*>(a.dw) + first * a.ldDw * elem;
+        const bool splitDx = plan.splitsDx > 1, splitDw = plan.splitsDw > 1;
+        int partsDx = 1, partsDw = 1;
         if (tc) {
             ceDzTensorCore(a, first, columns, dz, plan.ldDz, a.db == nullptr ? nullptr : biasPartials, stream);
-            if (a.dw != nullptr) ceDwTensorCore(a, first, columns, dz, plan.ldDz, stream);
-            if (a.dx != nullptr) ceDxTensorCore(a, first, columns, dz, plan.ldDz, dxOut, dxType, ldDxOut, addend, a.dim, stream);
+            if (a.dw != nullptr) {
+                if (splitDw) {
+                    ceDwTensorCore(a, columns, dz, plan.ldDz, parts, BFB_F32, a.dim, plan.splitsDw, stream);
+                    partsDw = partsOf(a.tokens, plan.splitsDw, 64);
+                } else {
+                    ceDwTensorCore(a, columns, dz, plan.ldDz, dwOut, a.gradDtype, a.ldDw, 1, stream);
+                }
+            }
         } else {
             CeSimtArgs p = simtOperands(a, first, columns);
             p.lse = a.lseIn;
@@ -443,7 +551,6 @@ void linearCeBackward(const LinearCeArgs& a, cudaStream_t stream) {
             p.gradScale = a.gradScale;
             p.dz = static_cast<float*>(dz);
             p.ldDz = plan.ldDz;
-            const bool f32 = a.dtype == BFB_F32;
             if (f32) ceSimtKernel<kSimtDz, float, float, float><<<simtGrid(p.m, p.n), 256, 0, stream>>>(p);
             else ceSimtKernel<kSimtDz, __nv_bfloat16, __nv_bfloat16, float><<<simtGrid(p.m, p.n), 256, 0, stream>>>(p);
             BFB_LAUNCH_CHECK();
@@ -453,45 +560,39 @@ void linearCeBackward(const LinearCeArgs& a, cudaStream_t stream) {
                 w.a = dz;
                 w.aRow = 1;
                 w.aDepth = plan.ldDz;
-                w.b = a.x;
                 w.bRow = 1;
                 w.bDepth = a.ldX;
                 w.m = columns;
                 w.n = a.dim;
                 w.k = a.tokens;
-                w.out = static_cast<uint8_t*>(a.dw) + first * a.ldDw * elem;
-                w.ldOut = a.ldDw;
-                const int grid = simtGrid(w.m, w.n);
-                if (f32 && elem == 4) ceSimtKernel<kSimtGrad, float, float, float><<<grid, 256, 0, stream>>>(w);
-                else if (f32) ceSimtKernel<kSimtGrad, float, float, __nv_bfloat16><<<grid, 256, 0, stream>>>(w);
-                else if (elem == 4) ceSimtKernel<kSimtGrad, float, __nv_bfloat16, float><<<grid, 256, 0, stream>>>(w);
-                else ceSimtKernel<kSimtGrad, float, __nv_bfloat16, __nv_bfloat16><<<grid, 256, 0, stream>>>(w);
-                BFB_LAUNCH_CHECK();
-                noteLaunch();
+                w.out = splitDw ? parts : dwOut;
+                w.ldOut = splitDw ? a.dim : a.ldDw;
+                partsDw = simtProduct(w, a.x, f32, splitDw ? BFB_F32 : a.gradDtype, plan.splitsDw);
             }
-            if (a.dx != nullptr) {   // dx(t, d) = sum_v dz(t, v) W(v, d)
+        }
+        if (a.dw != nullptr && splitDw) cePartSum(parts, partsDw, columns, a.dim, nullptr, 0, dwOut, a.gradDtype, a.ldDw, stream);
+        if (a.dx != nullptr) {   // dx(t, d) = sum_v dz(t, v) W(v, d)
+            if (tc) {
+                if (splitDx) ceDxTensorCore(a, first, columns, dz, plan.ldDz, parts, BFB_F32, a.dim, nullptr, 0, plan.splitsDx, stream);
+                else ceDxTensorCore(a, first, columns, dz, plan.ldDz, dxOut, dxType, ldDxOut, addend, a.dim, 1, stream);
+                partsDx = partsOf(columns, plan.splitsDx, 64);
+            } else {
                 CeSimtArgs x{};
                 x.a = dz;
                 x.aRow = plan.ldDz;
                 x.aDepth = 1;
-                x.b = p.b;
                 x.bRow = 1;
                 x.bDepth = a.ldW;
                 x.m = a.tokens;
                 x.n = a.dim;
                 x.k = columns;
-                x.out = dxOut;
-                x.ldOut = ldDxOut;
-                x.addend = addend;
+                x.out = splitDx ? parts : dxOut;
+                x.ldOut = splitDx ? a.dim : ldDxOut;
+                x.addend = splitDx ? nullptr : addend;
                 x.ldAddend = a.dim;
-                const int grid = simtGrid(x.m, x.n);
-                if (f32 && dxType == BFB_F32) ceSimtKernel<kSimtGrad, float, float, float><<<grid, 256, 0, stream>>>(x);
-                else if (f32) ceSimtKernel<kSimtGrad, float, float, __nv_bfloat16><<<grid, 256, 0, stream>>>(x);
-                else if (dxType == BFB_F32) ceSimtKernel<kSimtGrad, float, __nv_bfloat16, float><<<grid, 256, 0, stream>>>(x);
-                else ceSimtKernel<kSimtGrad, float, __nv_bfloat16, __nv_bfloat16><<<grid, 256, 0, stream>>>(x);
-                BFB_LAUNCH_CHECK();
-                noteLaunch();
+                partsDx = simtProduct(x, simtOperands(a, first, columns).b, f32, splitDx ? BFB_F32 : dxType, plan.splitsDx);
             }
+            if (splitDx) cePartSum(parts, partsDx, a.tokens, a.dim, addend, a.dim, dxOut, dxType, ldDxOut, stream);
         }
         if (a.db != nullptr) {
             const unsigned blocks = static_cast<unsigned>((columns + 31) / 32);

@@ -111,7 +111,7 @@ __device__ __forceinline__ void ceLogits(const uint32_t (&raw)[32], float (&v)[3
 template <int kMode, bool kAMn, bool kBMn, typename TC>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kCeThreads, 1)
 cePairKernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant__ CUtensorMap tmapB, const CeEpilogue ep, int m, int n,
-             int k, int tilesM, int tilesN, int groupN, int* status) {
+             int k, int tilesM, int tilesN, int groupN, int kPerSplit, int splits, int* status) {
     constexpr uint32_t kIdesc = make_idesc(kCePairM, 256, 1u, kBMn ? 1u : 0u) | (kAMn ? 1u << 15 : 0u);
 
     extern __shared__ uint8_t smemRaw[];
@@ -128,7 +128,8 @@ cePairKernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant__ 
     const uint32_t rank = cluster_ctarank();
     const bool leader = rank == 0;
     const int numK = (k + kCeBlockK - 1) / kCeBlockK;
-    const int totalTiles = tilesM * tilesN;
+    const int tiles = tilesM * tilesN;
+    const int totalTiles = tiles * splits;   // a tile's reduction in `splits` parts of kPerSplit stages
     const int clusterId = blockIdx.x >> 1;
     const int numClusters = gridDim.x >> 1;
 
@@ -162,10 +163,11 @@ cePairKernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant__ 
         uint32_t phase = 0;
         bool alive = true;
         for (int t = clusterId; t < totalTiles && alive; t += numClusters) {
-            const CeTile tc = ceTileCoord(t, tilesM, tilesN, groupN);
+            const CeTile tc = ceTileCoord(t % tiles, tilesM, tilesN, groupN);
             const int rowA = tc.m * kCePairM + static_cast<int>(rank) * 128;
             const int rowB = tc.n * kCeAccN + static_cast<int>(rank) * 128;
-            for (int kb = 0; kb < numK; ++kb) {
+            const int kBegin = t / tiles * kPerSplit, kEnd = min(numK, kBegin + kPerSplit);
+            for (int kb = kBegin; kb < kEnd; ++kb) {
                 if (!warp_all(mbar_wait(&emptyBar[stage], phase ^ 1u, abortFlag, status, kDevTimeoutStageEmpty))) {
                     alive = false;
                     break;
@@ -216,7 +218,8 @@ cePairKernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant__ 
                 if (!mbar_wait(&accEmptyBar[buf], accPhase ^ 1u, abortFlag, status, kDevTimeoutAccEmpty)) break;
                 tc_fence_after();
                 const uint32_t dTmem = tmemBase + static_cast<uint32_t>(buf * kCeAccN);
-                for (int kb = 0; kb < numK; ++kb) {
+                const int kBegin = t / tiles * kPerSplit, kEnd = min(numK, kBegin + kPerSplit);
+                for (int kb = kBegin; kb < kEnd; ++kb) {
                     if (!mbar_wait(&fullBar[stage], phase, abortFlag, status, kDevTimeoutTmaFull)) {
                         alive = false;
                         break;
@@ -226,10 +229,10 @@ cePairKernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant__ 
 #pragma unroll
                     for (int kk = 0; kk < kCeBlockK / 16; ++kk) {
                         umma_f16_pair_words(dTmem, a0 + offset + kk * kStepA, kHi, b0 + offset + kk * kStepB, kHi, kIdesc,
-                                            (kb > 0 || kk > 0) ? 1u : 0u);
+                                            (kb > kBegin || kk > 0) ? 1u : 0u);
                     }
                     umma_commit_pair(&emptyBar[stage]);
-                    if (kb == numK - 1) umma_commit_pair(&accFullBar[buf]);
+                    if (kb == kEnd - 1) umma_commit_pair(&accFullBar[buf]);
                     if (++stage == kCeStages) {
                         stage = 0;
                         phase ^= 1u;
@@ -245,7 +248,7 @@ cePairKernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant__ 
         uint8_t* stageTile = smem + kCeStages * kCeStageBytes + 256 + (warp - 4) * 4096;
         int local = 0;
         for (int t = clusterId; t < totalTiles; t += numClusters, ++local) {
-            const CeTile tc = ceTileCoord(t, tilesM, tilesN, groupN);
+            const CeTile tc = ceTileCoord(t % tiles, tilesM, tilesN, groupN);
             const int buf = local & 1;
             const uint32_t accPhase = static_cast<uint32_t>(local >> 1) & 1u;
             if (!warp_all(mbar_wait(&accFullBar[buf], accPhase, abortFlag, status, kDevTimeoutAccFull))) break;
@@ -338,7 +341,8 @@ cePairKernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant__ 
             } else {
                 constexpr int kRoundCols = 128 / static_cast<int>(sizeof(TC));
                 constexpr int kPieceCols = 16 / static_cast<int>(sizeof(TC));
-                TC* out = static_cast<TC*>(ep.out);
+                // a part of a split reduction goes to its own [m][ldOut] block
+                TC* out = static_cast<TC*>(ep.out) + static_cast<size_t>(t / tiles) * static_cast<size_t>(m) * static_cast<size_t>(ep.ldOut);
 #pragma unroll 1
                 for (int round = 0; round < 128 / kRoundCols; ++round) {
                     const int col0 = firstCol + round * kRoundCols;
@@ -418,20 +422,23 @@ void ceOperandMap(TensorMapStorage* out, const void* base, int64_t rows, int64_t
 }
 
 template <int kMode, bool kAMn, bool kBMn, typename TC>
-void launchCe(const TensorMapStorage& ta, const TensorMapStorage& tb, const CeEpilogue& ep, int64_t m, int64_t n, int64_t k, int* status,
-              cudaStream_t stream) {
+void launchCe(const TensorMapStorage& ta, const TensorMapStorage& tb, const CeEpilogue& ep, int64_t m, int64_t n, int64_t k, int splits,
+              int* status, cudaStream_t stream) {
     const int tilesM = static_cast<int>((m + kCePairM - 1) / kCePairM);
     const int tilesN = static_cast<int>((n + kCeAccN - 1) / kCeAccN);
     // about 4096 columns of B stay L2-resident while the rows sweep past (16 MB at a depth of 2048)
     const int groups = (tilesN + 15) / 16;
     const int groupN = (tilesN + groups - 1) / groups;
-    const int clusters = std::max(1, std::min(tilesM * tilesN, persistentSms() / 2));
+    const int stages = static_cast<int>((k + kCeBlockK - 1) / kCeBlockK);
+    const int kPerSplit = (stages + splits - 1) / splits;
+    splits = (stages + kPerSplit - 1) / kPerSplit;   // callers sized for this many parts (ceSplits)
+    const int clusters = std::max(1, std::min(tilesM * tilesN * splits, persistentSms() / 2));
     auto kernel = cePairKernel<kMode, kAMn, kBMn, TC>;
     BFB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kCeSmemBytes));
     ProfileScope prof(kProfGemmTc, stream, 2.0 * static_cast<double>(m) * static_cast<double>(n) * static_cast<double>(k));
     kernel<<<2 * clusters, kCeThreads, kCeSmemBytes, stream>>>(*reinterpret_cast<const CUtensorMap*>(ta.bytes),
                                                                *reinterpret_cast<const CUtensorMap*>(tb.bytes), ep, static_cast<int>(m),
-                                                               static_cast<int>(n), static_cast<int>(k), tilesM, tilesN, groupN, status);
+                                                               static_cast<int>(n), static_cast<int>(k), tilesM, tilesN, groupN, kPerSplit, splits, status);
     BFB_LAUNCH_CHECK();
     noteLaunch();
 }
@@ -448,7 +455,7 @@ void ceStatsTensorCore(const LinearCeArgs& a, float2* partials, float* labelLogi
     ep.vocab = a.vocab;
     ep.partials = partials;
     ep.labelLogit = labelLogit;
-    launchCe<kCeStats, false, false, float>(tx, tw, ep, a.tokens, a.vocab, a.dim, a.dStatus, stream);
+    launchCe<kCeStats, false, false, float>(tx, tw, ep, a.tokens, a.vocab, a.dim, 1, a.dStatus, stream);
 }
 
 void ceDzTensorCore(const LinearCeArgs& a, int64_t firstColumn, int64_t columns, void* dz, int64_t ldDz, float* biasPartials,
@@ -468,11 +475,29 @@ void ceDzTensorCore(const LinearCeArgs& a, int64_t firstColumn, int64_t columns,
     ep.dz = static_cast<__nv_bfloat16*>(dz);
     ep.ldDz = ldDz;
     ep.biasPartials = biasPartials;
-    launchCe<kCeDz, false, false, float>(tx, tw, ep, a.tokens, columns, a.dim, a.dStatus, stream);
+    launchCe<kCeDz, false, false, float>(tx, tw, ep, a.tokens, columns, a.dim, 1, a.dStatus, stream);
+}
+
+int ceSplits(int64_t m, int64_t n, int64_t k) {
+    const int64_t tiles = ((m + kCePairM - 1) / kCePairM) * ((n + kCeAccN - 1) / kCeAccN);
+    const int64_t stages = (k + kCeBlockK - 1) / kCeBlockK;
+    // 74 pairs whatever the device has free: the split decides how sums are grouped, and results do not depend on that
+    constexpr int64_t kPairs = 74;
+    int best = 1;
+    double cost = static_cast<double>((tiles + kPairs - 1) / kPairs);
+    for (int s = 2; s <= 16 && stages / s >= 16; ++s) {
+        const double c = static_cast<double>((tiles * s + kPairs - 1) / kPairs) / s;
+        if (c < 0.9 * cost) {
+            best = s;
+            cost = c;
+        }
+    }
+    const int64_t per = (stages + best - 1) / best;
+    return static_cast<int>((stages + per - 1) / per);
 }
 
 void ceDxTensorCore(const LinearCeArgs& a, int64_t firstColumn, int64_t columns, const void* dz, int64_t ldDz, void* out, int outDtype,
-                    int64_t ldOut, const float* addend, int64_t ldAddend, cudaStream_t stream) {
+                    int64_t ldOut, const float* addend, int64_t ldAddend, int splits, cudaStream_t stream) {
     TensorMapStorage tz, tw;
     ceOperandMap(&tz, dz, a.tokens, columns, ldDz, false);
     ceOperandMap(&tw, static_cast<const __nv_bfloat16*>(a.w) + firstColumn * a.ldW, columns, a.dim, a.ldW, true);
@@ -481,23 +506,20 @@ void ceDxTensorCore(const LinearCeArgs& a, int64_t firstColumn, int64_t columns,
     ep.ldOut = ldOut;
     ep.addend = addend;
     ep.ldAddend = ldAddend;
-    if (outDtype == BFB_F32) launchCe<kCeGrad, false, true, float>(tz, tw, ep, a.tokens, a.dim, columns, a.dStatus, stream);
-    else launchCe<kCeGrad, false, true, __nv_bfloat16>(tz, tw, ep, a.tokens, a.dim, columns, a.dStatus, stream);
+    if (outDtype == BFB_F32) launchCe<kCeGrad, false, true, float>(tz, tw, ep, a.tokens, a.dim, columns, splits, a.dStatus, stream);
+    else launchCe<kCeGrad, false, true, __nv_bfloat16>(tz, tw, ep, a.tokens, a.dim, columns, splits, a.dStatus, stream);
 }
 
-void ceDwTensorCore(const LinearCeArgs& a, int64_t firstColumn, int64_t columns, const void* dz, int64_t ldDz, cudaStream_t stream) {
+void ceDwTensorCore(const LinearCeArgs& a, int64_t columns, const void* dz, int64_t ldDz, void* out, int outDtype, int64_t ldOut, int splits,
+                    cudaStream_t stream) {
     TensorMapStorage tz, tx;
     ceOperandMap(&tz, dz, a.tokens, columns, ldDz, true);
     ceOperandMap(&tx, a.x, a.tokens, a.dim, a.ldX, true);
     CeEpilogue ep;
-    ep.ldOut = a.ldDw;
-    if (a.gradDtype == BFB_F32) {
-        ep.out = static_cast<float*>(a.dw) + firstColumn * a.ldDw;
-        launchCe<kCeGrad, true, true, float>(tz, tx, ep, columns, a.dim, a.tokens, a.dStatus, stream);
-    } else {
-        ep.out = static_cast<__nv_bfloat16*>(a.dw) + firstColumn * a.ldDw;
-        launchCe<kCeGrad, true, true, __nv_bfloat16>(tz, tx, ep, columns, a.dim, a.tokens, a.dStatus, stream);
-    }
+    ep.out = out;
+    ep.ldOut = ldOut;
+    if (outDtype == BFB_F32) launchCe<kCeGrad, true, true, float>(tz, tx, ep, columns, a.dim, a.tokens, splits, a.dStatus, stream);
+    else launchCe<kCeGrad, true, true, __nv_bfloat16>(tz, tx, ep, columns, a.dim, a.tokens, splits, a.dStatus, stream);
 }
 
 }  // namespace bfb

@@ -127,7 +127,8 @@ def make(torch, tokens, vocab, dim, dtype, with_bias, seed, pad=0, spread=2.0):
 
 
 TC_SHAPES = [(1, 1, 8), (1, 300, 64), (2, 127, 16), (7, 257, 64), (33, 128, 72), (128, 256, 64), (129, 1000, 136), (256, 4097, 256),
-             (300, 1003, 200), (515, 777, 512), (1030, 2500, 64)]
+             (300, 1003, 200), (515, 777, 512), (1030, 2500, 64), (5000, 300, 64),
+             (300, 20001, 200)]
 
 
 @pytest.mark.parametrize("tokens,vocab,dim", TC_SHAPES)
