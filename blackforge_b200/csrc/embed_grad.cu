@@ -114,6 +114,7 @@ struct SortBuffers {
 __global__ void __launch_bounds__(kSortThreads, 1)
 sortTokensKernel(const float* __restrict__ ids, SortBuffers buf, uint32_t* __restrict__ occurs, int64_t count, int64_t vocab, int passes, int bits,
                  int cluster) {
+    pdl_launch_dependents();   // the reduction may set itself up; it waits for the sorted lists
     extern __shared__ uint32_t counts[];   // [kSortWarps][bins], then [bins] totals of this block, [bins] bases
     const int bins = 1 << bits;
     uint32_t* blockTotal = counts + kSortWarps * bins;
@@ -286,6 +287,8 @@ __device__ __forceinline__ void storeRow(T* row, int64_t pack, const float (&acc
 template <typename TIn, typename TOut, int kN>
 __global__ void __launch_bounds__(kReduceThreads)
 embedReduceKernel(const ReduceParams p) {
+    pdl_launch_dependents();
+    pdl_wait();
     __shared__ uint32_t sKey[kMaxPiece + 2], sValue[kMaxPiece];
     const int64_t reduceBlocks = p.pieces * p.columnBlocks;
     const int tid = threadIdx.x;
@@ -396,6 +399,7 @@ embedReduceKernel(const ReduceParams p) {
 template <typename TOut>
 __global__ void __launch_bounds__(256)
 embedJoinKernel(const ReduceParams p) {
+    pdl_wait();
     const int64_t piece = blockIdx.x;
     const int64_t begin = piece * p.piece, next = begin + p.piece;   // piece + 1 < pieces: `next` is an entry
     const uint32_t key = p.keys[next - 1], following = p.keys[next], first = p.keys[begin], earlier = begin > 0 ? p.keys[begin - 1] : 0xFFFFFFFFu;
@@ -472,13 +476,13 @@ void launchReduce(ReduceParams p, cudaStream_t stream) {
     const int64_t zeroBlocks = p.accumulate ? 0 : (p.vocab + kZeroRows - 1) / kZeroRows;
     const int64_t blocks = p.pieces * p.columnBlocks + zeroBlocks;
     if (blocks > 0) {
-        embedReduceKernel<TIn, TOut, kN><<<static_cast<unsigned>(blocks), kReduceThreads, 0, stream>>>(p);
+        launchDependent(embedReduceKernel<TIn, TOut, kN>, dim3(static_cast<unsigned>(blocks)), dim3(kReduceThreads), 0, stream, p);
         BFB_LAUNCH_CHECK();
         noteLaunch();
     }
     if (p.pieces > 1) {
         const dim3 grid(static_cast<unsigned>(p.pieces - 1), static_cast<unsigned>((p.dim + 255) / 256));
-        embedJoinKernel<TOut><<<grid, 256, 0, stream>>>(p);
+        launchDependent(embedJoinKernel<TOut>, grid, dim3(256), 0, stream, p);
         BFB_LAUNCH_CHECK();
         noteLaunch();
     }

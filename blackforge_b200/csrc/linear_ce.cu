@@ -23,6 +23,7 @@
 #include "common.cuh"
 #include "kernels.hpp"
 #include "linear_ce.cuh"
+#include "ptx_sm100.cuh"
 
 namespace bfb {
 
@@ -79,6 +80,8 @@ enum { kSimtStats = 0, kSimtDz = 1, kSimtGrad = 2 };
 // memory, not its arithmetic.
 template <int kMode, typename TA, typename TB, typename TC>
 __global__ void __launch_bounds__(256, 2) ceSimtKernel(const CeSimtArgs p) {
+    pdl_launch_dependents();
+    pdl_wait();
     __shared__ alignas(16) float sa[kDepth][kTile + 4];
     __shared__ alignas(16) float sb[kDepth][kTile + 4];
     __shared__ float2 rowStat[kTile][16];
@@ -197,6 +200,8 @@ __global__ void __launch_bounds__(256, 2) ceSimtKernel(const CeSimtArgs p) {
 __global__ void __launch_bounds__(1024)
 ceFinishKernel(const float2* __restrict__ partials, int64_t parts, const float* __restrict__ labelLogit, const float* __restrict__ labels,
                int64_t vocab, float* loss, float* lse, int64_t tokens, int* oobCount) {
+    pdl_launch_dependents();
+    pdl_wait();
     __shared__ float2 joined[32][33];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const int64_t row = static_cast<int64_t>(blockIdx.x) * 32 + lane;
@@ -234,6 +239,8 @@ ceFinishKernel(const float2* __restrict__ partials, int64_t parts, const float* 
 // {sum of the losses, rows that count, 1 / rows that count}: one block, a fixed order, the sum in 64 bits.
 __global__ void __launch_bounds__(1024)
 ceSummaryKernel(const float* __restrict__ loss, const float* __restrict__ labels, int64_t vocab, int64_t tokens, float* summary) {
+    pdl_launch_dependents();
+    pdl_wait();
     __shared__ double sums[32];
     __shared__ unsigned long long counts[32];
     double sum = 0.0;
@@ -277,6 +284,8 @@ ceSummaryKernel(const float* __restrict__ loss, const float* __restrict__ labels
 // Column sums of `rows` rows of partial sums (or of dz itself): 32 columns per block, the rows split over eight warps.
 __global__ void __launch_bounds__(256)
 ceColumnSumKernel(const float* __restrict__ in, int64_t ld, int64_t rows, int64_t columns, float* out) {
+    pdl_launch_dependents();
+    pdl_wait();
     __shared__ float joined[8][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t col = static_cast<int64_t>(blockIdx.x) * 32 + lane;
@@ -296,6 +305,8 @@ template <typename TC>
 __global__ void __launch_bounds__(256)
 cePartSumKernel(const float* __restrict__ parts, int splits, int64_t rows, int64_t cols, const float* addend, int64_t ldAddend, TC* out,
                 int64_t ldOut) {
+    pdl_launch_dependents();
+    pdl_wait();
     const int64_t total = rows * cols, step = static_cast<int64_t>(gridDim.x) * blockDim.x;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += step) {
         const int64_t row = i / cols, col = i - row * cols;
@@ -316,8 +327,8 @@ cePartSumKernel(const float* __restrict__ parts, int splits, int64_t rows, int64
 void cePartSum(const float* parts, int splits, int64_t rows, int64_t cols, const float* addend, int64_t ldAddend, void* out, int outDtype,
                int64_t ldOut, cudaStream_t stream) {
     const int grid = static_cast<int>(std::min<int64_t>((rows * cols + 255) / 256, static_cast<int64_t>(smCount()) * 16));
-    if (outDtype == BFB_F32) cePartSumKernel<float><<<grid, 256, 0, stream>>>(parts, splits, rows, cols, addend, ldAddend, static_cast<float*>(out), ldOut);
-    else cePartSumKernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(parts, splits, rows, cols, addend, ldAddend, static_cast<__nv_bfloat16*>(out), ldOut);
+    if (outDtype == BFB_F32) launchDependent(cePartSumKernel<float>, dim3(grid), dim3(256), 0, stream, parts, splits, rows, cols, addend, ldAddend, static_cast<float*>(out), ldOut);
+    else launchDependent(cePartSumKernel<__nv_bfloat16>, dim3(grid), dim3(256), 0, stream, parts, splits, rows, cols, addend, ldAddend, static_cast<__nv_bfloat16*>(out), ldOut);
     BFB_LAUNCH_CHECK();
     noteLaunch();
 }
@@ -460,20 +471,20 @@ void linearCeForward(const LinearCeArgs& a, cudaStream_t stream) {
             p.partials = partials;
             p.labelLogit = labelLogit;
             const int grid = simtGrid(p.m, p.n);
-            if (a.dtype == BFB_F32) ceSimtKernel<kSimtStats, float, float, float><<<grid, 256, 0, stream>>>(p);
-            else ceSimtKernel<kSimtStats, __nv_bfloat16, __nv_bfloat16, float><<<grid, 256, 0, stream>>>(p);
+            if (a.dtype == BFB_F32) launchDependent(ceSimtKernel<kSimtStats, float, float, float>, dim3(grid), dim3(256), 0, stream, p);
+            else launchDependent(ceSimtKernel<kSimtStats, __nv_bfloat16, __nv_bfloat16, float>, dim3(grid), dim3(256), 0, stream, p);
             BFB_LAUNCH_CHECK();
             noteLaunch();
         }
         // a warp of 32 rows for every four parts, up to 32 of them
         const int finishThreads = static_cast<int>(std::min<int64_t>(32, (plan.parts + 3) / 4)) * 32;
-        ceFinishKernel<<<static_cast<unsigned>((a.tokens + 31) / 32), finishThreads, 0, stream>>>(partials, plan.parts, labelLogit, a.labels, a.vocab,
+        launchDependent(ceFinishKernel, dim3(static_cast<unsigned>((a.tokens + 31) / 32)), dim3(finishThreads), 0, stream, partials, plan.parts, labelLogit, a.labels, a.vocab,
                                                                                       a.loss, a.lse, a.tokens, a.oobCount);
         BFB_LAUNCH_CHECK();
         noteLaunch();
     }
     if (a.summary != nullptr) {
-        ceSummaryKernel<<<1, 1024, 0, stream>>>(a.loss, a.labels, a.vocab, a.tokens, a.summary);
+        launchDependent(ceSummaryKernel, dim3(1), dim3(1024), 0, stream, a.loss, a.labels, a.vocab, a.tokens, a.summary);
         BFB_LAUNCH_CHECK();
         noteLaunch();
     }
@@ -509,10 +520,10 @@ void linearCeBackward(const LinearCeArgs& a, cudaStream_t stream) {
         g.b = b;
         g.kPerSplit = (g.k + splits - 1) / splits;
         const dim3 grid(simtGrid(g.m, g.n), static_cast<unsigned>((g.k + g.kPerSplit - 1) / g.kPerSplit));
-        if (bIsF32 && outDtype == BFB_F32) ceSimtKernel<kSimtGrad, float, float, float><<<grid, 256, 0, stream>>>(g);
-        else if (bIsF32) ceSimtKernel<kSimtGrad, float, float, __nv_bfloat16><<<grid, 256, 0, stream>>>(g);
-        else if (outDtype == BFB_F32) ceSimtKernel<kSimtGrad, float, __nv_bfloat16, float><<<grid, 256, 0, stream>>>(g);
-        else ceSimtKernel<kSimtGrad, float, __nv_bfloat16, __nv_bfloat16><<<grid, 256, 0, stream>>>(g);
+        if (bIsF32 && outDtype == BFB_F32) launchDependent(ceSimtKernel<kSimtGrad, float, float, float>, dim3(grid), dim3(256), 0, stream, g);
+        else if (bIsF32) launchDependent(ceSimtKernel<kSimtGrad, float, float, __nv_bfloat16>, dim3(grid), dim3(256), 0, stream, g);
+        else if (outDtype == BFB_F32) launchDependent(ceSimtKernel<kSimtGrad, float, __nv_bfloat16, float>, dim3(grid), dim3(256), 0, stream, g);
+        else launchDependent(ceSimtKernel<kSimtGrad, float, __nv_bfloat16, __nv_bfloat16>, dim3(grid), dim3(256), 0, stream, g);
         BFB_LAUNCH_CHECK();
         noteLaunch();
         return static_cast<int>(grid.y);
@@ -551,8 +562,8 @@ void linearCeBackward(const LinearCeArgs& a, cudaStream_t stream) {
             p.gradScale = a.gradScale;
             p.dz = static_cast<float*>(dz);
             p.ldDz = plan.ldDz;
-            if (f32) ceSimtKernel<kSimtDz, float, float, float><<<simtGrid(p.m, p.n), 256, 0, stream>>>(p);
-            else ceSimtKernel<kSimtDz, __nv_bfloat16, __nv_bfloat16, float><<<simtGrid(p.m, p.n), 256, 0, stream>>>(p);
+            if (f32) launchDependent(ceSimtKernel<kSimtDz, float, float, float>, dim3(simtGrid(p.m, p.n)), dim3(256), 0, stream, p);
+            else launchDependent(ceSimtKernel<kSimtDz, __nv_bfloat16, __nv_bfloat16, float>, dim3(simtGrid(p.m, p.n)), dim3(256), 0, stream, p);
             BFB_LAUNCH_CHECK();
             noteLaunch();
             if (a.dw != nullptr) {   // dW(v, d) = sum_t dz(t, v) x(t, d)
@@ -596,8 +607,8 @@ void linearCeBackward(const LinearCeArgs& a, cudaStream_t stream) {
         }
         if (a.db != nullptr) {
             const unsigned blocks = static_cast<unsigned>((columns + 31) / 32);
-            if (tc) ceColumnSumKernel<<<blocks, 256, 0, stream>>>(biasPartials, plan.ldDz, (a.tokens + 31) / 32, columns, a.db + first);
-            else ceColumnSumKernel<<<blocks, 256, 0, stream>>>(static_cast<const float*>(dz), plan.ldDz, a.tokens, columns, a.db + first);
+            if (tc) launchDependent(ceColumnSumKernel, dim3(blocks), dim3(256), 0, stream, biasPartials, plan.ldDz, (a.tokens + 31) / 32, columns, a.db + first);
+            else launchDependent(ceColumnSumKernel, dim3(blocks), dim3(256), 0, stream, static_cast<const float*>(dz), plan.ldDz, a.tokens, columns, a.db + first);
             BFB_LAUNCH_CHECK();
             noteLaunch();
         }

@@ -133,6 +133,7 @@ cePairKernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant__ 
     const int clusterId = blockIdx.x >> 1;
     const int numClusters = gridDim.x >> 1;
 
+    pdl_launch_dependents();   // the next kernel of the step may set itself up; it waits for this one's results
     if (threadIdx.x == 0) {
         for (int s = 0; s < kCeStages; ++s) {
             mbar_init(&fullBar[s], 1);
@@ -156,6 +157,7 @@ cePairKernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant__ 
     cluster_sync_all();  // both CTAs' barriers exist before any remote arrival or copy can reach them
     tc_fence_after();
     const uint32_t tmemBase = *tmemSlot;
+    pdl_wait();   // nothing of the kernel before is read, and nothing it reads overwritten, before here
 
     if (warp == 0) {
         // ---------------- TMA producer (both CTAs) ----------------
@@ -436,9 +438,9 @@ void launchCe(const TensorMapStorage& ta, const TensorMapStorage& tb, const CeEp
     auto kernel = cePairKernel<kMode, kAMn, kBMn, TC>;
     BFB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kCeSmemBytes));
     ProfileScope prof(kProfGemmTc, stream, 2.0 * static_cast<double>(m) * static_cast<double>(n) * static_cast<double>(k));
-    kernel<<<2 * clusters, kCeThreads, kCeSmemBytes, stream>>>(*reinterpret_cast<const CUtensorMap*>(ta.bytes),
-                                                               *reinterpret_cast<const CUtensorMap*>(tb.bytes), ep, static_cast<int>(m),
-                                                               static_cast<int>(n), static_cast<int>(k), tilesM, tilesN, groupN, kPerSplit, splits, status);
+    launchDependent(kernel, dim3(2 * clusters), dim3(kCeThreads), kCeSmemBytes, stream, *reinterpret_cast<const CUtensorMap*>(ta.bytes),
+                    *reinterpret_cast<const CUtensorMap*>(tb.bytes), ep, static_cast<int>(m), static_cast<int>(n), static_cast<int>(k), tilesM,
+                    tilesN, groupN, kPerSplit, splits, status);
     BFB_LAUNCH_CHECK();
     noteLaunch();
 }
