@@ -484,7 +484,7 @@ void distillTopk(const DistillArgs& a, cudaStream_t stream) {
     require(a.rows >= 0 && a.vocab > 0 && a.k > 0, "distill_topk: sizes must be positive");
     require(a.vocab <= (1ll << 24) && a.rows <= (1ll << 27), "distill_topk: sizes beyond the limits (2^27 rows, 2^24 classes)");
     require(a.k <= kMaxTeacher, "distill_topk: more than 1024 teacher entries a row");
-    require(a.tau > 0.0f && a.tau < INFINITY, "distill_topk: the temperature must be positive and finite");
+    require(a.tau >= 1e-6f && a.tau <= 1e6f, "distill_topk: the temperature must be within 1e-6 .. 1e6");
     require(a.ldLogits >= a.vocab && (a.grad == nullptr || a.ldGrad >= a.vocab), "distill_topk: row pitch smaller than vocab");
     if (a.rows == 0) return;
     require(a.logits != nullptr && a.ids != nullptr && a.teacher != nullptr, "distill_topk: null pointer");

@@ -102,9 +102,10 @@ embedScaledKernel(const float* __restrict__ ids, const TIn* __restrict__ table, 
 
 // ---- 1. sort -------------------------------------------------------------------------------------------------
 
+// (row, token position) in one word of eight bytes: a place in the sorted list costs one scattered store, and those are what a
+// pass of the sort is made of.
 struct SortBuffers {
-    uint32_t* keys[2];
-    uint32_t* values[2];
+    uint2* pairs[2];
 };
 
 // Stable radix sort of (row, position) pairs, `passes` digits of `bits` bits. The cluster's blocks, their warps and a
@@ -126,46 +127,51 @@ sortTokensKernel(const float* __restrict__ ids, SortBuffers buf, uint32_t* __res
     const int64_t begin = min(count, (static_cast<int64_t>(rank) * kSortWarps + warp) * perWarp);
     const int64_t end = min(count, begin + perWarp);
     uint32_t* mine = counts + warp * bins;
+    // warps of this block that have a stretch
+    const int64_t before0 = static_cast<int64_t>(rank) * kSortWarps * perWarp;
+    const int active = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(kSortWarps), (count - before0 + perWarp - 1) / perWarp)));
     const int64_t all32 = static_cast<int64_t>(cluster) * kSortThreads, me = static_cast<int64_t>(rank) * kSortThreads + tid;
     for (int64_t i = me; i < (vocab + 31) / 32; i += all32) occurs[i] = 0;
     constexpr int kBatch = 8;   // loads in flight per lane
     for (int pass = 0; pass < passes; ++pass) {
         const int shift = pass * bits;
-        const uint32_t* srcKeys = buf.keys[(pass & 1) ^ 1];
-        const uint32_t* srcValues = buf.values[(pass & 1) ^ 1];
-        uint32_t* dstKeys = buf.keys[pass & 1];
-        uint32_t* dstValues = buf.values[pass & 1];
-        // the stretch's keys from i0 on, a batch per lane; all loads first, whatever lies behind the end reads the last one again
-        auto keysAt = [&](int64_t i0, uint32_t (&key)[kBatch]) {
-            uint32_t raw[kBatch];
+        const uint2* src = buf.pairs[(pass & 1) ^ 1];
+        uint2* dst = buf.pairs[pass & 1];
+        // the stretch's pairs from i0 on, a batch per lane; all loads first, whatever lies behind the end reads the last one again
+        auto pairsAt = [&](int64_t i0, uint2 (&pair)[kBatch]) {
+            if (pass == 0) {
+                float id[kBatch];
 #pragma unroll
-            for (int u = 0; u < kBatch; ++u) {
-                const int64_t i = min(i0 + 32 * u + lane, end - 1);
-                raw[u] = pass == 0 ? __float_as_uint(__ldg(ids + i)) : __ldcg(srcKeys + i);
+                for (int u = 0; u < kBatch; ++u) id[u] = __ldg(ids + min(i0 + 32 * u + lane, end - 1));
+#pragma unroll
+                for (int u = 0; u < kBatch; ++u) pair[u] = make_uint2(tokenRow(id[u], vocab), static_cast<uint32_t>(i0 + 32 * u + lane));
+            } else {
+#pragma unroll
+                for (int u = 0; u < kBatch; ++u) pair[u] = __ldcg(src + min(i0 + 32 * u + lane, end - 1));
             }
-#pragma unroll
-            for (int u = 0; u < kBatch; ++u) key[u] = pass == 0 ? tokenRow(__uint_as_float(raw[u]), vocab) : raw[u];
         };
-        for (int i = tid; i < kSortWarps * bins; i += kSortThreads) counts[i] = 0;
+        for (int i = tid; i < active * bins; i += kSortThreads) counts[i] = 0;
         __syncthreads();
         for (int64_t i0 = begin; i0 < end; i0 += 32 * kBatch) {
-            uint32_t key[kBatch];
-            keysAt(i0, key);
+            uint2 pair[kBatch];
+            pairsAt(i0, pair);
 #pragma unroll
             for (int u = 0; u < kBatch; ++u)
-                if (i0 + 32 * u + lane < end) atomicAdd(&mine[(key[u] >> shift) & (bins - 1)], 1u);
+                if (i0 + 32 * u + lane < end) atomicAdd(&mine[(pair[u].x >> shift) & (bins - 1)], 1u);
         }
         __syncthreads();
         // per digit: what the block's earlier warps hold, and the block's total
         if (tid < bins) {
-            uint32_t held[kSortWarps];
-#pragma unroll
-            for (int w = 0; w < kSortWarps; ++w) held[w] = counts[w * bins + tid];
             uint32_t total = 0;
+            for (int w0 = 0; w0 < active; w0 += 8) {
+                uint32_t held[8];
 #pragma unroll
-            for (int w = 0; w < kSortWarps; ++w) {
-                counts[w * bins + tid] = total;
-                total += held[w];
+                for (int w = 0; w < 8; ++w) held[w] = w0 + w < active ? counts[(w0 + w) * bins + tid] : 0;
+#pragma unroll
+                for (int w = 0; w < 8; ++w) {
+                    if (w0 + w < active) counts[(w0 + w) * bins + tid] = total;
+                    total += held[w];
+                }
             }
             blockTotal[tid] = total;
         }
@@ -203,26 +209,18 @@ sortTokensKernel(const float* __restrict__ ids, SortBuffers buf, uint32_t* __res
         __syncthreads();
         // places, 32 pairs at a time
         for (int64_t i0 = begin; i0 < end; i0 += 32 * kBatch) {
-            uint32_t keys[kBatch], values[kBatch];
-            keysAt(i0, keys);
-#pragma unroll
-            for (int u = 0; u < kBatch; ++u) {
-                const int64_t i = min(i0 + 32 * u + lane, end - 1);
-                values[u] = pass == 0 ? static_cast<uint32_t>(i) : __ldcg(srcValues + i);
-            }
+            uint2 pair[kBatch];
+            pairsAt(i0, pair);
 #pragma unroll
             for (int u = 0; u < kBatch; ++u) {
                 if (i0 + 32 * u >= end) break;
                 const bool live = i0 + 32 * u + lane < end;
-                const uint32_t digit = live ? (keys[u] >> shift) & (bins - 1) : 0xFFFFFFFFu;
+                const uint32_t digit = live ? (pair[u].x >> shift) & (bins - 1) : 0xFFFFFFFFu;
                 const uint32_t same = __match_any_sync(0xFFFFFFFFu, digit);
                 if (live) {
                     const uint32_t earlier = __popc(same & ((1u << lane) - 1u));
                     const uint32_t at = base[digit] + mine[digit] + earlier;
-                    if (at < count) {   // always, unless the ids change while the kernel runs
-                        dstKeys[at] = keys[u];
-                        dstValues[at] = values[u];
-                    }
+                    if (at < count) dst[at] = pair[u];   // always, unless the ids change while the kernel runs
                 }
                 __syncwarp();
                 if (live && lane == 31 - __clz(same)) mine[digit] += __popc(same);
@@ -235,14 +233,14 @@ sortTokensKernel(const float* __restrict__ ids, SortBuffers buf, uint32_t* __res
         else __syncthreads();
     }
     // where a run begins: its row occurs
-    const uint32_t* sorted = buf.keys[(passes - 1) & 1];
+    const uint2* sorted = buf.pairs[(passes - 1) & 1];
     for (int64_t i0 = me; i0 < count; i0 += all32 * 4) {
         uint32_t key[4], before[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const int64_t i = i0 + u * all32;
-            key[u] = i < count ? __ldcg(sorted + i) : static_cast<uint32_t>(vocab);
-            before[u] = i > 0 && i < count ? __ldcg(sorted + i - 1) : 0xFFFFFFFFu;
+            key[u] = i < count ? __ldcg(&sorted[i].x) : static_cast<uint32_t>(vocab);
+            before[u] = i > 0 && i < count ? __ldcg(&sorted[i - 1].x) : 0xFFFFFFFFu;
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u)
@@ -253,8 +251,7 @@ sortTokensKernel(const float* __restrict__ ids, SortBuffers buf, uint32_t* __res
 // ---- 2. sums of the sorted rows ---------------------------------------------------------------------------------
 
 struct ReduceParams {
-    const uint32_t* keys;      // sorted rows
-    const uint32_t* values;    // token positions
+    const uint2* pairs;        // sorted (row, token position)
     const uint32_t* occurs;    // a bit for every row that is named (null: none is)
     int64_t count;             // entries, those that name no row last
     int64_t vocab, dim;
@@ -301,8 +298,9 @@ embedReduceKernel(const ReduceParams p) {
         const uint32_t none = static_cast<uint32_t>(p.vocab);
         if (tid < n + 2) {
             const int64_t i = begin + tid - 1;
-            sKey[tid] = i >= 0 && i < p.count ? p.keys[i] : none;
-            if (tid >= 1 && tid <= n) sValue[tid - 1] = p.values[i];
+            const uint2 pair = i >= 0 && i < p.count ? p.pairs[i] : make_uint2(none, 0);
+            sKey[tid] = pair.x;
+            if (tid >= 1 && tid <= n) sValue[tid - 1] = pair.y;
         }
         __syncthreads();
         if (pack * kN >= p.dim) return;
@@ -402,7 +400,7 @@ embedJoinKernel(const ReduceParams p) {
     pdl_wait();
     const int64_t piece = blockIdx.x;
     const int64_t begin = piece * p.piece, next = begin + p.piece;   // piece + 1 < pieces: `next` is an entry
-    const uint32_t key = p.keys[next - 1], following = p.keys[next], first = p.keys[begin], earlier = begin > 0 ? p.keys[begin - 1] : 0xFFFFFFFFu;
+    const uint32_t key = p.pairs[next - 1].x, following = p.pairs[next].x, first = p.pairs[begin].x, earlier = begin > 0 ? p.pairs[begin - 1].x : 0xFFFFFFFFu;
     if (key >= p.vocab || following != key) return;       // nothing goes on
     if (first == key && earlier == key) return;           // the chain started earlier
     const int64_t col = static_cast<int64_t>(blockIdx.y) * blockDim.x + threadIdx.x;
@@ -412,7 +410,7 @@ embedJoinKernel(const ReduceParams p) {
     constexpr int kAhead = 16;
     float sum = p.ends[(piece * 2 + 1) * p.dim + col];
     const float second = p.ends[(piece + 1) * 2 * p.dim + col];
-    const uint32_t third = p.keys[min(piece + 2, p.pieces - 1) * p.piece];
+    const uint32_t third = p.pairs[min(piece + 2, p.pieces - 1) * p.piece].x;
     sum += second;
     if (piece + 2 < p.pieces && third == key) {
         for (int64_t q = piece + 2;; q += kAhead) {
@@ -421,7 +419,7 @@ embedJoinKernel(const ReduceParams p) {
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
                 const int64_t at = min(q + u, p.pieces - 1);
-                keys[u] = p.keys[at * p.piece];
+                keys[u] = p.pairs[at * p.piece].x;
                 part[u] = p.ends[at * 2 * p.dim + col];
             }
             bool more = true;
@@ -570,16 +568,12 @@ void embedScaledBackward(const float* ids, const void* dout, int doutDtype, int6
     if (tokens > 0) {
         auto* base = static_cast<uint8_t*>(workspace);
         SortBuffers buf;
-        for (int i = 0; i < 2; ++i) {
-            buf.keys[i] = reinterpret_cast<uint32_t*>(base + (2 * i) * need.list);
-            buf.values[i] = reinterpret_cast<uint32_t*>(base + (2 * i + 1) * need.list);
-        }
+        for (int i = 0; i < 2; ++i) buf.pairs[i] = reinterpret_cast<uint2*>(base + 2 * i * need.list);
         p.ends = reinterpret_cast<float*>(base + 4 * need.list);
         auto* occurs = reinterpret_cast<uint32_t*>(base + 4 * need.list + need.ends);
         p.occurs = occurs;
         const SortPlan s = sortPlan(tokens, vocab);
-        p.keys = buf.keys[(s.passes - 1) & 1];
-        p.values = buf.values[(s.passes - 1) & 1];
+        p.pairs = buf.pairs[(s.passes - 1) & 1];
         const size_t smem = static_cast<size_t>(kSortWarps + 2) * (1u << s.bits) * 4;
         BFB_CUDA(cudaFuncSetAttribute(sortTokensKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
         cudaLaunchConfig_t cfg = {};

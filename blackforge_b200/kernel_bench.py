@@ -6,6 +6,9 @@ run, on small cases.
     python -m blackforge_b200.kernel_bench attention --batch 16 --heads 16 --seq 2048
     python -m blackforge_b200.kernel_bench attention-bwd --batch 8 --heads 16 --seq 2048
     python -m blackforge_b200.kernel_bench matmul-bwd --m 65536 --k 2048 --n 5632
+    python -m blackforge_b200.kernel_bench linear-ce --rows 16384 --vocab 32000 --dim 2048 [--forward-only]
+    python -m blackforge_b200.kernel_bench embed-scaled --rows 65536 --vocab 32000 --dim 2048
+    python -m blackforge_b200.kernel_bench distill --rows 8192 --vocab 32000 --k 64
     python -m blackforge_b200.kernel_bench rmsnorm --rows 65536 --dim 2048
     python -m blackforge_b200.kernel_bench embed --batch 32 --seq 2048 --vocab 32000 --dim 2048
 
@@ -24,7 +27,8 @@ import numpy as np
 
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("kernel", choices=["gemm", "attention", "attention-bwd", "matmul-bwd", "rmsnorm", "embed", "checkpoint"])
+    ap.add_argument("kernel", choices=["gemm", "attention", "attention-bwd", "matmul-bwd", "linear-ce", "embed-scaled", "distill",
+                                       "rmsnorm", "embed", "checkpoint"])
     ap.add_argument("--layers", type=int, default=4)
     ap.add_argument("--hidden", type=int, default=5632)
     ap.add_argument("--chunk-mib", type=int, default=0, help="checkpoint: staging buffer size (0: the loader's default)")
@@ -43,6 +47,7 @@ def main():
     ap.add_argument("--dim", type=int, default=2048)
     ap.add_argument("--vocab", type=int, default=32000)
     ap.add_argument("--stream-dtype", default="bf16", choices=["bf16", "f32"])
+    ap.add_argument("--forward-only", action="store_true", help="linear-ce: the loss without its gradient")
     ap.add_argument("--iters", type=int, default=10)
     ap.add_argument("--warmup", type=int, default=3)
     ap.add_argument("--no-flush", action="store_true")
@@ -146,6 +151,53 @@ def main():
             bfb.check(lib.bfb_matmul_bf16_backward(a.ptr, b.ptr, g.ptr, d_a.ptr, d_b.ptr, args.m, args.k, args.n, None))
         work, unit = 4.0 * args.m * args.k * args.n, "TFLOP/s"
         desc = {"m": args.m, "k": args.k, "n": args.n, "operands": "fp32 in, bf16 products, fp32 out", "flops": "dA and dB"}
+    elif args.kernel == "linear-ce":
+        # loss of the output projection (mean over the rows) and, by default, the gradients of x and W in bf16
+        x, w = rand_dev(args.rows * args.dim, bfb.BF16), rand_dev(args.vocab * args.dim, bfb.BF16, 2.0 / args.dim ** 0.5)
+        labels = bfb.DeviceBuffer.from_numpy(rng.integers(0, args.vocab, size=args.rows).astype(np.float32))
+        size = workspace(bfb, lib.bfb_linear_cross_entropy_workspace, bfb.BF16, args.rows, args.vocab, args.dim, int(not args.forward_only))
+        ws = bfb.DeviceBuffer(size)
+        loss, lse, summary = bfb.DeviceBuffer(args.rows * 4), bfb.DeviceBuffer(args.rows * 4), bfb.DeviceBuffer(12)
+        dx, dw = bfb.DeviceBuffer(args.rows * args.dim * 2), bfb.DeviceBuffer(args.vocab * args.dim * 2)
+
+        def run():
+            bfb.check(lib.bfb_linear_cross_entropy_fwd(x.ptr, args.dim, w.ptr, args.dim, None, labels.ptr, loss.ptr, lse.ptr, summary.ptr,
+                                                       bfb.BF16, args.rows, args.vocab, args.dim, None, ws.ptr, size, status.ptr, None))
+            if not args.forward_only:
+                bfb.check(lib.bfb_linear_cross_entropy_bwd(x.ptr, args.dim, w.ptr, args.dim, None, labels.ptr, lse.ptr, None,
+                                                           summary.ptr + 8, 1.0, dx.ptr, args.dim, dw.ptr, args.dim, None, bfb.BF16,
+                                                           bfb.BF16, args.rows, args.vocab, args.dim, ws.ptr, size, status.ptr, None))
+        work, unit = (2.0 if args.forward_only else 8.0) * args.rows * args.vocab * args.dim, "TFLOP/s"
+        desc = {"rows": args.rows, "vocab": args.vocab, "dim": args.dim, "workspace_bytes": size,
+                "flops": "one product" if args.forward_only else "four products: the logits twice, dx, dW"}
+    elif args.kernel == "embed-scaled":
+        # fp32 table: lookup, then the table's gradient by sorted tokens (frequencies that fall with the rank)
+        ids = bfb.DeviceBuffer.from_numpy(np.minimum(np.floor(np.exp(rng.random(args.rows) * np.log(args.vocab + 1.0))) - 1,
+                                                     args.vocab - 1).astype(np.float32))
+        table, dout = rand_dev(args.vocab * args.dim, bfb.F32), rand_dev(args.rows * args.dim, bfb.F32)
+        out, dtable = bfb.DeviceBuffer(args.rows * args.dim * 4), bfb.DeviceBuffer(args.vocab * args.dim * 4)
+        size = workspace(bfb, lib.bfb_embed_scaled_bwd_workspace, args.rows, args.vocab, args.dim)
+        ws = bfb.DeviceBuffer(size)
+
+        def run():
+            bfb.check(lib.bfb_embed_scaled(ids.ptr, table.ptr, bfb.F32, out.ptr, bfb.F32, args.dim, args.rows, args.vocab, args.dim,
+                                           args.dim ** 0.5, None, None))
+            bfb.check(lib.bfb_embed_scaled_bwd(ids.ptr, dout.ptr, bfb.F32, args.dim, dtable.ptr, bfb.F32, args.rows, args.vocab,
+                                               args.dim, args.dim ** 0.5, 0, ws.ptr, size, None))
+        work, unit = float((2 * args.rows + args.vocab + min(args.rows, args.vocab)) * args.dim * 4), "GB/s"
+        desc = {"rows": args.rows, "vocab": args.vocab, "dim": args.dim}
+    elif args.kernel == "distill":
+        # fp32 logits in, loss and fp32 gradient out
+        k = min(args.k, 1024, args.vocab)
+        z, dz = rand_dev(args.rows * args.vocab, bfb.F32, 2.5), bfb.DeviceBuffer(args.rows * args.vocab * 4)
+        ids = bfb.DeviceBuffer.from_numpy(rng.integers(0, args.vocab, size=(args.rows, k)).astype(np.float32))
+        teacher, loss, lse = rand_dev(args.rows * k, bfb.F32), bfb.DeviceBuffer(args.rows * 4), bfb.DeviceBuffer(args.rows * 4)
+
+        def run():
+            bfb.check(lib.bfb_distill_topk(z.ptr, bfb.F32, args.vocab, ids.ptr, teacher.ptr, bfb.F32, k, 2.0, None, None, 1.0, loss.ptr,
+                                           lse.ptr, dz.ptr, bfb.F32, args.vocab, args.rows, args.vocab, None, None))
+        work, unit = float(args.rows * args.vocab * 8), "GB/s"
+        desc = {"rows": args.rows, "vocab": args.vocab, "k": k}
     elif args.kernel == "rmsnorm":
         sd = bfb.BF16 if args.stream_dtype == "bf16" else bfb.F32
         x = rand_dev(args.rows * args.dim, sd)
@@ -187,6 +239,13 @@ def main():
     print(json.dumps({"kernel": args.kernel, "case": desc, "ms_median": ms, "ms_min": float(min(times)), "rate": rate,
                       "unit": unit, "iters": args.iters, "l2_flushed": flush is not None, "device_status": st}))
     return 0 if st == 0 else 1
+
+
+def workspace(bfb, query, *sizes):
+    import ctypes
+    n = ctypes.c_size_t(0)
+    bfb.check(query(*sizes, ctypes.byref(n)))
+    return n.value
 
 
 def checkpoint_io(args, bfb):

@@ -329,6 +329,7 @@ bfb_status bfb_attention_bwd(const void* d_dout, const void* d_q, const void* d_
  * the vocabulary's gradient of z (tokens x piece, at most 256 MiB or 4096 columns) and fp32 sums of dx; its pointer has to be
  * 256-byte aligned. Nothing in it has to survive from call to call, and nothing of it is kept: calls that may run at the
  * same time (other streams, two captured graphs) take one each.
+ * Results may not overlap operands: a piece's gradients are written while x and W are still needed.
  * _fwd writes d_loss [tokens] (may be NULL), d_lse [tokens] and, when d_summary is not NULL, {sum of the losses, rows that
  * count, 1 / rows that count (0 if none)}.
  * _bwd takes the same operands and d_lse, and the gradient of each row's loss as grad_scale * *d_grad_scale *
@@ -376,7 +377,7 @@ bfb_status bfb_embed_scaled_bwd(const float* d_ids, const void* d_dout, int32_t 
  *   d_dlogits[t, j] = g_t * temperature * (p_j - sum of q_k over the entries with id_k = j)
  * with g_t = grad_scale * *d_grad_scale * d_grad_loss[t] (device operands may be NULL, standing for 1).
  *  d_logits [rows, vocab] BFB_F32 or BFB_BF16, pitch ld_logits, any alignment; d_teacher_ids [rows, k] float32 holding
- *  integers; d_teacher_logits [rows, k] BFB_F32 or BFB_BF16; 1 <= k <= 1024. An entry with a negative id or a teacher
+ *  integers; d_teacher_logits [rows, k] BFB_F32 or BFB_BF16; 1 <= k <= 1024; 1e-6 <= temperature <= 1e6. An entry with a negative id or a teacher
  *  logit of -inf is left out; one at or above vocab, or not finite, too, and is counted in *d_oob_count (optional). An id
  *  may be listed more than once. A row without an entry has loss 0 and gradient 0. Student logits of -inf have
  *  probability 0 (an entry there with q > 0 makes the loss +inf); a row of nothing but -inf, or with NaN or +inf, has loss

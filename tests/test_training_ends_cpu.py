@@ -92,7 +92,7 @@ DISTILL = dict(z=4096, dtype=0, ld=10, ids=4096, teacher=4096, teacher_dtype=0, 
 
 
 @pytest.mark.parametrize("change", [dict(z=None), dict(ids=None), dict(teacher=None), dict(dtype=2), dict(teacher_dtype=2), dict(grad_dtype=2),
-                                    dict(ld=9), dict(ld_grad=9), dict(k=0), dict(k=1025), dict(tau=0.0), dict(tau=-1.0), dict(tau=float("nan")),
+                                    dict(ld=9), dict(ld_grad=9), dict(k=0), dict(k=1025), dict(tau=0.0), dict(tau=-1.0), dict(tau=1e-7), dict(tau=1e7), dict(tau=float("nan")),
                                     dict(tau=float("inf")), dict(rows=-1), dict(vocab=0), dict(vocab=(1 << 24) + 1, ld=1 << 25, ld_grad=1 << 25),
                                     dict(grad=4096, grad_dtype=1), dict(grad=4096, ld_grad=11)])
 def test_distill_refuses(bfb, change):
