@@ -389,7 +389,7 @@ int simtSplits(int64_t m, int64_t n, int64_t k) {
 }
 
 // The piece is as wide as its dz stays within 256 MiB, at least 4096 columns (narrower pieces make the dx product so
-// shallow that the fp32 sums it carries from piece to piece cost more than its MMAs), all pieces equally wide.
+// shallow that the fp32 sums it carries from piece to piece cost more than its MMAs).
 CePlan cePlan(int64_t tokens, int64_t vocab, int64_t dim, bool tensorCores) {
     CePlan p;
     p.tensorCores = tensorCores;
@@ -399,8 +399,21 @@ CePlan cePlan(int64_t tokens, int64_t vocab, int64_t dim, bool tensorCores) {
     p.parts = (vocab + part - 1) / part;
     const int64_t rows = std::max<int64_t>(tokens, 1);
     const int64_t widest = std::max<int64_t>(4096, kCeDzBytes / (elem * rows) / tile * tile);
-    p.pieces = (vocab + widest - 1) / widest;
-    p.pieceColumns = roundUp((vocab + p.pieces - 1) / p.pieces, tile);
+    const int64_t vocabTiles = (vocab + tile - 1) / tile;
+    int64_t width = std::min(widest / tile, vocabTiles);
+    if (tensorCores && width < vocabTiles) {
+        // dW's tiles of a piece go over 74 CTA pairs in waves, and a last wave that is nearly empty costs as much as a full
+        // one: of the widths down to half the widest, the one with the fewest waves in all (a quarter of a wave for a piece more)
+        const int64_t across = (dim + 255) / 256;
+        auto waves = [&](int64_t w) {
+            const int64_t whole = vocabTiles / w, rest = vocabTiles % w;
+            return static_cast<double>(whole * ((w * across + 73) / 74) + (rest * across + 73) / 74) + 0.25 * static_cast<double>(whole + (rest > 0));
+        };
+        const int64_t most = width;
+        for (int64_t w = most - 1; w >= (most + 1) / 2; --w)
+            if (waves(w) < waves(width)) width = w;
+    }
+    p.pieceColumns = width * tile;
     p.pieces = (vocab + p.pieceColumns - 1) / p.pieceColumns;
     p.ldDz = p.pieceColumns;
     p.forwardBytes = static_cast<size_t>(roundUp(p.parts * rows * 8, 256) + roundUp(rows * 4, 256));

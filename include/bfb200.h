@@ -326,8 +326,8 @@ bfb_status bfb_attention_bwd(const void* d_dout, const void* d_q, const void* d_
  *  do not count, too: they meet their zero gradient in the product that gives dW.
  *  d_status (optional int32 on device) as for bfb_gemm.
  * _workspace: bytes of the caller's workspace for a forward (backward == 0) or for both directions. It holds one piece of
- * the vocabulary's gradient of z (tokens x piece, at most 256 MiB or 4096 columns) and fp32 sums of dx; its pointer has to be
- * 256-byte aligned. Nothing in it has to survive from call to call, and nothing of it is kept: calls that may run at the
+ * the vocabulary's gradient of z (tokens x piece, at most 256 MiB or 4096 columns), fp32 sums of dx where there are several
+ * pieces, and the fp32 parts of gradient products whose reduction is split; its pointer has to be 256-byte aligned. Nothing in it has to survive from call to call, and nothing of it is kept: calls that may run at the
  * same time (other streams, two captured graphs) take one each.
  * Results may not overlap operands: a piece's gradients are written while x and W are still needed.
  * _fwd writes d_loss [tokens] (may be NULL), d_lse [tokens] and, when d_summary is not NULL, {sum of the losses, rows that
