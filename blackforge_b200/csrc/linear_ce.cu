@@ -281,9 +281,9 @@ ceSummaryKernel(const float* __restrict__ loss, const float* __restrict__ labels
     summary[2] = count == 0 ? 0.0f : static_cast<float>(1.0 / static_cast<double>(count));
 }
 
-// Column sums of `rows` rows of partial sums (or of dz itself): 32 columns per block, the rows split over eight warps.
+// Column sums of `rows` rows of partial sums (or of dz itself), times a factor: 32 columns per block, the rows split over eight warps.
 __global__ void __launch_bounds__(256)
-ceColumnSumKernel(const float* __restrict__ in, int64_t ld, int64_t rows, int64_t columns, float* out) {
+ceColumnSumKernel(const float* __restrict__ in, int64_t ld, int64_t rows, int64_t columns, const float* dScale, float scale, float* out) {
     pdl_launch_dependents();
     pdl_wait();
     __shared__ float joined[8][32];
@@ -297,7 +297,7 @@ ceColumnSumKernel(const float* __restrict__ in, int64_t ld, int64_t rows, int64_
     __syncthreads();
     if (warp != 0 || col >= columns) return;
     for (int w = 1; w < 8; ++w) sum += joined[w][lane];
-    out[col] = sum;
+    out[col] = sum * ceScale(dScale, scale);
 }
 
 // out = sum of the parts of a split product, in order, + addend.
@@ -620,8 +620,8 @@ void linearCeBackward(const LinearCeArgs& a, cudaStream_t stream) {
         }
         if (a.db != nullptr) {
             const unsigned blocks = static_cast<unsigned>((columns + 31) / 32);
-            if (tc) launchDependent(ceColumnSumKernel, dim3(blocks), dim3(256), 0, stream, biasPartials, plan.ldDz, (a.tokens + 31) / 32, columns, a.db + first);
-            else launchDependent(ceColumnSumKernel, dim3(blocks), dim3(256), 0, stream, static_cast<const float*>(dz), plan.ldDz, a.tokens, columns, a.db + first);
+            if (tc) launchDependent(ceColumnSumKernel, dim3(blocks), dim3(256), 0, stream, biasPartials, plan.ldDz, (a.tokens + 31) / 32, columns, a.dGradScale, a.gradScale, a.db + first);
+            else launchDependent(ceColumnSumKernel, dim3(blocks), dim3(256), 0, stream, static_cast<const float*>(dz), plan.ldDz, a.tokens, columns, nullptr, 1.0f, a.db + first);
             BFB_LAUNCH_CHECK();
             noteLaunch();
         }

@@ -22,9 +22,11 @@ __device__ __forceinline__ bool ceLabelIsBad(float label, int64_t vocab) {
     return static_cast<int64_t>(lroundf(label)) >= vocab;
 }
 
+__device__ __forceinline__ float ceScale(const float* dGradScale, float gradScale) {
+    return dGradScale != nullptr ? gradScale * *dGradScale : gradScale;
+}
 __device__ __forceinline__ float ceRowGrad(const float* gradLoss, int64_t row, const float* dGradScale, float gradScale) {
-    float g = gradScale;
-    if (dGradScale != nullptr) g *= *dGradScale;
+    float g = ceScale(dGradScale, gradScale);
     if (gradLoss != nullptr) g *= gradLoss[row];
     return g;
 }

@@ -4,9 +4,11 @@
 //
 //   kCeStats  z = x W^T + b per tile; each row's running maximum and sum of exponentials over the tile's columns
 //             go to a small array (one pair per row and 128 columns), the label's logit to one word per row
-//   kCeDz     the same product; the epilogue stores dz = g (exp(z - lse) - [column = label]) in bf16 for one piece of
-//             the vocabulary, and column sums of the unrounded dz per 32 rows for the bias gradient
-//   kCeGrad   the products with dz: dx += dz W (B operand with its reduction along rows) and dW = dz^T x (both
+//   kCeDz     the same product; the epilogue stores dz = w (exp(z - lse) - [column = label]) in bf16 for one piece of
+//             the vocabulary, and column sums of the unrounded dz per 32 rows for the bias gradient. w is the row's own
+//             weight only: a factor common to all rows (1 / rows) would give the label's entries, all near -1, one and
+//             the same rounding error, which the sums over rows and columns cannot average away
+//   kCeGrad   the products with dz times that common factor: dx += dz W (B operand with its reduction along rows) and dW = dz^T x (both
 //             operands that way). The MN-major operand forms of tcgen05 read the tiles as they lie in memory, so
 //             nothing is transposed by a pass of its own.
 //
@@ -67,12 +69,12 @@ struct CeEpilogue {
     float* labelLogit = nullptr;      // [tokens]
     const float* lse = nullptr;       // [tokens]
     const float* gradLoss = nullptr;  // [tokens] or null
-    const float* dGradScale = nullptr;
-    float gradScale = 1.0f;
     __nv_bfloat16* dz = nullptr;      // [tokens][ldDz]
     int64_t ldDz = 0;
     float* biasPartials = nullptr;    // [ceil(tokens / 32)][ldDz] or null
     // kCeGrad
+    const float* dGradScale = nullptr;  // one word or null
+    float gradScale = 1.0f;
     void* out = nullptr;              // [m][ldOut]
     int64_t ldOut = 0;
     const float* addend = nullptr;    // fp32 [m][ldAddend], or null: the sum over the pieces before this one
@@ -287,7 +289,7 @@ cePairKernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant__ 
                 int64_t label = -1;
                 if (rowOk) {
                     label = ceLabel(ep.labels[row], ep.vocab);
-                    if (label >= 0) g = ceRowGrad(ep.gradLoss, row, ep.dGradScale, ep.gradScale);
+                    if (label >= 0) g = ep.gradLoss != nullptr ? ep.gradLoss[row] : 1.0f;
                     label -= ep.firstColumn;
                     lse = ep.lse[row];
                 }
@@ -341,6 +343,7 @@ cePairKernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant__ 
                     __syncwarp();
                 }
             } else {
+                const float scale = ceScale(ep.dGradScale, ep.gradScale);   // the factor dz left out
                 constexpr int kRoundCols = 128 / static_cast<int>(sizeof(TC));
                 constexpr int kPieceCols = 16 / static_cast<int>(sizeof(TC));
                 // a part of a split reduction goes to its own [m][ldOut] block
@@ -359,7 +362,7 @@ cePairKernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant__ 
                             const int col = col0 + sub * 32 + g * 8;
                             float v[8];
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(raw[g * 8 + j]);
+                            for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(raw[g * 8 + j]) * scale;
                             if (ep.addend != nullptr && rowOk && col + 8 <= n) {
                                 const float4* r = reinterpret_cast<const float4*>(ep.addend + static_cast<size_t>(row) * static_cast<size_t>(ep.ldAddend) + col);
                                 const float4 r0 = r[0], r1 = r[1];
@@ -472,8 +475,6 @@ void ceDzTensorCore(const LinearCeArgs& a, int64_t firstColumn, int64_t columns,
     ep.firstColumn = firstColumn;
     ep.lse = a.lseIn;
     ep.gradLoss = a.gradLoss;
-    ep.dGradScale = a.dGradScale;
-    ep.gradScale = a.gradScale;
     ep.dz = static_cast<__nv_bfloat16*>(dz);
     ep.ldDz = ldDz;
     ep.biasPartials = biasPartials;
@@ -508,6 +509,8 @@ void ceDxTensorCore(const LinearCeArgs& a, int64_t firstColumn, int64_t columns,
     ceOperandMap(&tz, dz, a.tokens, columns, ldDz, false);
     ceOperandMap(&tw, static_cast<const __nv_bfloat16*>(a.w) + firstColumn * a.ldW, columns, a.dim, a.ldW, true);
     CeEpilogue ep;
+    ep.dGradScale = a.dGradScale;
+    ep.gradScale = a.gradScale;
     ep.out = out;
     ep.ldOut = ldOut;
     ep.addend = addend;
@@ -522,6 +525,8 @@ void ceDwTensorCore(const LinearCeArgs& a, int64_t columns, const void* dz, int6
     ceOperandMap(&tz, dz, a.tokens, columns, ldDz, true);
     ceOperandMap(&tx, a.x, a.tokens, a.dim, a.ldX, true);
     CeEpilogue ep;
+    ep.dGradScale = a.dGradScale;
+    ep.gradScale = a.gradScale;
     ep.out = out;
     ep.ldOut = ldOut;
     if (outDtype == BFB_F32) launchCe<kCeGrad, true, true, float>(tz, tx, ep, columns, a.dim, a.tokens, splits, a.dStatus, stream);
