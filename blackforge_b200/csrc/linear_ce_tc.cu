@@ -12,6 +12,12 @@
 //             operands that way). The MN-major operand forms of tcgen05 read the tiles as they lie in memory, so
 //             nothing is transposed by a pass of its own.
 //
+// Bound by the tensor pipe: of the measured cuBLAS rate the statistics reach 100 % (4096 x 32000 x 2048 in 0.323 ms), dz 98 %
+// (16384 x 8192 x 2048 in 0.340 ms), dW 89 - 95 % and dx 95 % of it in isolation; a whole step of 16384 x 32000 x 2048 takes 5.5 ms
+// (1555 TFLOP/s over its four products), 6.5 ms where steps follow each other and the power limit sets the clock. The tile is
+// the 256 x 256 of a pair because its operands (64 B/clk read by the MMAs, 64 B/clk written by TMA) just fit the shared memory's
+// bandwidth; an epilogue of two exponentials per logit and a row's 128 columns hides under a tile's MMAs from a depth of about 512.
+//
 // Roles, rings and barriers are those of the plain CTA-pair GEMM (gemm_tc2.cu): a TMA producer warp per CTA, one MMA
 // issuer in the leader CTA, eight epilogue warps per CTA on double-buffered accumulators.
 #include <cuda.h>

@@ -327,16 +327,17 @@ bfb_status bfb_attention_bwd(const void* d_dout, const void* d_q, const void* d_
  *  d_status (optional int32 on device) as for bfb_gemm.
  * _workspace: bytes of the caller's workspace for a forward (backward == 0) or for both directions. It holds one piece of
  * the vocabulary's gradient of z (tokens x piece, at most 256 MiB or 4096 columns), fp32 sums of dx where there are several
- * pieces, and the fp32 parts of gradient products whose reduction is split; its pointer has to be 256-byte aligned. Nothing in it has to survive from call to call, and nothing of it is kept: calls that may run at the
- * same time (other streams, two captured graphs) take one each.
+ * pieces, and the fp32 parts of gradient products whose reduction is split; its pointer has to be 256-byte aligned. Nothing
+ * in it has to survive from call to call, and nothing of it is kept: calls that may run at the same time (other streams,
+ * two captured graphs) take one each.
  * Results may not overlap operands: a piece's gradients are written while x and W are still needed.
  * _fwd writes d_loss [tokens] (may be NULL), d_lse [tokens] and, when d_summary is not NULL, {sum of the losses, rows that
  * count, 1 / rows that count (0 if none)}.
  * _bwd takes the same operands and d_lse, and the gradient of each row's loss as grad_scale * *d_grad_scale *
  * d_grad_loss[t] (the two device operands may be NULL, standing for 1): d_grad_scale = d_summary + 2 gives the mean's
  * gradient. Each of d_dx [tokens, dim], d_dw [vocab, dim] (grad_dtype BFB_F32 or BFB_BF16, pitches ld_dx, ld_dw) and
- * d_dbias f32 [vocab] may be NULL and is overwritten otherwise. On the tensor-core route the gradient of z is rounded to bf16
- * once, as the operand of the two products (dbias sums the unrounded values). */
+ * d_dbias f32 [vocab] may be NULL and is overwritten otherwise. On the tensor-core route the gradient of z, without
+ * the factors common to all rows, is rounded to bf16 once as the operand of the two products (dbias sums the unrounded values). */
 bfb_status bfb_linear_cross_entropy_workspace(int32_t dtype, int64_t tokens, int64_t vocab, int64_t dim, int32_t backward,
                                               size_t* bytes);
 bfb_status bfb_linear_cross_entropy_fwd(const void* d_x, int64_t ld_x, const void* d_w, int64_t ld_w, const float* d_bias,
@@ -377,11 +378,11 @@ bfb_status bfb_embed_scaled_bwd(const float* d_ids, const void* d_dout, int32_t 
  *   d_dlogits[t, j] = g_t * temperature * (p_j - sum of q_k over the entries with id_k = j)
  * with g_t = grad_scale * *d_grad_scale * d_grad_loss[t] (device operands may be NULL, standing for 1).
  *  d_logits [rows, vocab] BFB_F32 or BFB_BF16, pitch ld_logits, any alignment; d_teacher_ids [rows, k] float32 holding
- *  integers; d_teacher_logits [rows, k] BFB_F32 or BFB_BF16; 1 <= k <= 1024; 1e-6 <= temperature <= 1e6. An entry with a negative id or a teacher
- *  logit of -inf is left out; one at or above vocab, or not finite, too, and is counted in *d_oob_count (optional). An id
- *  may be listed more than once. A row without an entry has loss 0 and gradient 0. Student logits of -inf have
- *  probability 0 (an entry there with q > 0 makes the loss +inf); a row of nothing but -inf, or with NaN or +inf, has loss
- *  and gradient NaN.
+ *  integers; d_teacher_logits [rows, k] BFB_F32 or BFB_BF16; 1 <= k <= 1024; 1e-6 <= temperature <= 1e6. An entry with a
+ *  negative id or a teacher logit of -inf is left out; one at or above vocab, or not finite, too, and is counted in
+ *  *d_oob_count (optional). An id may be listed more than once. A row without an entry has loss 0 and gradient 0. Student
+ *  logits of -inf have probability 0 (an entry there with q > 0 makes the loss +inf); a row of nothing but -inf, or with NaN
+ *  or +inf, has loss and gradient NaN.
  *  d_loss, d_lse (log sum exp of d_logits / temperature) and d_dlogits (grad_dtype BFB_F32 or BFB_BF16, pitch
  *  ld_dlogits) may each be NULL. d_dlogits may be d_logits itself (same format and pitch), but not overlap it otherwise.
  *  Everything is summed in fp32 in an order that depends on the sizes and on where a row starts in a 16-byte line only. */
